@@ -370,6 +370,142 @@ MAC_API int mac_decode_rope_preserve_q_bf16(void* q, int64_t q_stride0, void* k,
                                             int32_t cache_locs_is_i64, int64_t N, int32_t Hq, int32_t Hkv,
                                             int32_t head_dim, int32_t is_neox, void* stream);
 
+/* ------------------------------------------------------ paged 8-bit cache --- */
+
+/* Element type of a paged cache besides MAC_DTYPE_BF16 / MAC_DTYPE_F16: OCP
+ * e4m3 codes (no infinities). */
+enum { MAC_DTYPE_E4M3 = 3 };
+
+/*
+ * A paged K/V cache (no reference counterpart; its pool is bf16 with pages of
+ * one token).  Row (page, slot, head) of K starts at k_cache + page *
+ * k_page_stride + slot * k_slot_stride + head * k_head_stride (BYTES, likewise
+ * V), its D elements are contiguous: pages [page_size, Hkv, D] or [Hkv,
+ * page_size, D], K and V apart or interleaved, the bf16 pool of the other
+ * entry points (page_size 1).  Strides are multiples of 16 bytes, base pointers
+ * 16-byte aligned; page_size is a power of two.
+ *
+ * e4m3 caches: with kv_scales (u8 [num_pages, Hkv, page_size, 2], contiguous,
+ * 2-byte aligned) a row of K or V has its own E8M0 byte e and an element is
+ * code * 2^(e - 127) (e = 255: NaN); k_scale and v_scale are then 1.  With
+ * kv_scales NULL an element is code * k_scale or code * v_scale (both > 0).
+ * 16-bit caches have kv_scales NULL, and K and V count times k_scale and
+ * v_scale as well (1 for plain rows).
+ */
+typedef struct MacPagedCache {
+  uint32_t struct_size; /* sizeof(MacPagedCache) */
+  uint32_t abi_version; /* MAC_ABI_VERSION */
+  void* k_cache;
+  void* v_cache;
+  void* kv_scales; /* or NULL */
+  int64_t num_pages;
+  int64_t k_page_stride, k_slot_stride, k_head_stride; /* bytes */
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int32_t page_size, Hkv, D;
+  int32_t cache_dtype; /* MAC_DTYPE_E4M3, or MAC_DTYPE_BF16 / MAC_DTYPE_F16 (attention only) */
+  float k_scale, v_scale;
+} MacPagedCache;
+
+/* Writes tokens rows k, v (dtype MAC_DTYPE_BF16 / MAC_DTYPE_F16; token and head
+ * strides in elements, D contiguous elements, any alignment) quantised into an
+ * e4m3 cache: token n to slot cache_locs[n] = page * page_size + slot (i32 or
+ * i64); locs outside the cache (negative: padding) are skipped.  Row-scaled
+ * form: the row's scale is the smallest power of two s >= 2^-126 with max |x|
+ * <= 448 s over its finite elements; static form: x / k_scale, saturated.
+ * Codes round to nearest even; NaN and infinities become NaN.  D: multiples of
+ * 16 up to 256.  Two tokens of one call must not name the same slot: its row
+ * and scale would be one token's or the other's, element by element. */
+MAC_API int mac_paged_cache_write_fp8(const MacPagedCache* cache, const void* k, int64_t k_stride0, int64_t k_stride1,
+                                      const void* v, int64_t v_stride0, int64_t v_stride1, int32_t dtype,
+                                      const void* cache_locs, int32_t cache_locs_is_i64, int64_t tokens,
+                                      void* stream);
+
+/* Decode RoPE with that write (the 8-bit counterpart of
+ * mac_decode_rope_preserve_q_bf16): q_out[n] = RoPE(q[n]) ([tokens, Hq, D],
+ * contiguous, 16-byte aligned; q itself is left as it is, the pre-RoPE query),
+ * and RoPE(k[n]) (fp32, quantised without another rounding) and v[n] go to
+ * slot cache_locs[n].  RoPE, cos_sin_cache, positions and is_neox as in
+ * mac_decode_rope_preserve_q_bf16. */
+typedef struct MacPagedRopeArgs {
+  uint32_t struct_size; /* sizeof(MacPagedRopeArgs) */
+  uint32_t abi_version; /* MAC_ABI_VERSION */
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_stride0, q_stride1, k_stride0, k_stride1, v_stride0, v_stride1; /* elements */
+  void* q_out;
+  const float* cos_sin_cache;
+  int64_t cos_sin_rows, cos_sin_stride0;
+  const void* positions;
+  const void* cache_locs;
+  int64_t tokens;
+  int32_t Hq, rotary_dim, is_neox;
+  int32_t dtype;
+  int32_t positions_is_i64, cache_locs_is_i64;
+} MacPagedRopeArgs;
+
+MAC_API int mac_paged_rope_write_fp8(const MacPagedCache* cache, const MacPagedRopeArgs* args, void* stream);
+
+/* Reads rows back: out_k[i], out_v[i] ([rows, Hkv, D] of dtype MAC_DTYPE_F32 /
+ * BF16 / F16, contiguous, 16-byte aligned) are the values of slot
+ * kv_indices[i]; slots outside the cache read as zeros.  Exact in fp32 and,
+ * row-scaled, in bf16 (subnormals of 2^-126 scales aside); otherwise rounded to
+ * nearest even. */
+MAC_API int mac_paged_cache_read_fp8(const MacPagedCache* cache, const void* kv_indices, int32_t kv_indices_is_i64,
+                                     int64_t rows, void* out_k, void* out_v, int32_t dtype, void* stream);
+
+/*
+ * Attention of a chunk of new tokens over a paged cache (no reference
+ * counterpart; the reference leaves it to its serving engine): one token per
+ * request (decode), a few (drafted tokens), or a prefill chunk, ragged.
+ * Request b owns query rows [qo_indptr[b], qo_indptr[b+1]) and kv_lens[b]
+ * cached keys, the new tokens' among them: row i of n sits at position pos =
+ * kv_len - n + i and attends to the keys at [max(pos - window_left, 0), pos]
+ * (window_left < 0: [0, pos]).  Key t lies in page page_table[row][t /
+ * page_size], slot t % page_size, with row = req_ids[b] (req_ids NULL: b).
+ *   s = q . k sm_scale, or logit_cap tanh(q . k sm_scale / logit_cap) for
+ *   logit_cap > 0; out = softmax(s) V; out_lse = log sum e^s (natural log).
+ * Keys past the table, or in pages outside [0, num_pages), are masked (V there
+ * may hold anything); rows that see no key (kv_len < n, a table row outside the
+ * table) get 0 and -inf.  Requests whose rows are not within [0, total_q) are
+ * skipped, and rows of no request are not written; requests must not share
+ * rows.
+ *   q       [total_q, Hq, D] of q_dtype (MAC_DTYPE_BF16 / F16), token and head
+ *           strides in elements, rows 16-byte aligned
+ *   cache   of q_dtype or MAC_DTYPE_E4M3; D 64, 128 or 256; any group size
+ *   out     [total_q, Hq, D] of q_dtype, out_lse f32 [total_q, Hq], contiguous
+ *   page_table i32 [table_rows, table_cols], rows table_stride entries apart
+ * Sums are fp32; weights are rounded to q_dtype for their product with V.  A
+ * call's results depend on its inputs and shapes only.
+ */
+typedef struct MacPagedAttentionArgs {
+  uint32_t struct_size; /* sizeof(MacPagedAttentionArgs) */
+  uint32_t abi_version; /* MAC_ABI_VERSION */
+  const void* q;
+  int64_t q_stride0, q_stride1;
+  const int32_t* qo_indptr; /* [B+1] */
+  const int32_t* kv_lens;   /* [B] */
+  const int32_t* page_table;
+  int64_t table_stride;
+  const int32_t* req_ids; /* [B] or NULL */
+  void* out;
+  float* out_lse;
+  int64_t total_q;
+  int32_t B, Hq;
+  int32_t table_rows, table_cols;
+  int32_t q_dtype;
+  int32_t window_left;
+  double sm_scale, logit_cap;
+} MacPagedAttentionArgs;
+
+/* The workspace (16-byte aligned, any content, the caller's until the call's
+ * work on `stream` is done; calls that overlap need one each) has the bytes
+ * that mac_paged_chunk_attention_workspace names for the same shapes, on the
+ * same device (0: none; -1: bad arguments).  Pointers are not looked at there. */
+MAC_API int64_t mac_paged_chunk_attention_workspace(const MacPagedCache* cache, const MacPagedAttentionArgs* args);
+MAC_API int mac_paged_chunk_attention(const MacPagedCache* cache, const MacPagedAttentionArgs* args, void* workspace,
+                                      int64_t workspace_bytes, void* stream);
+
 /* Message of the last failed call on this thread ("" if none).  No reference
  * counterpart: the reference raises through TORCH_CHECK instead. */
 MAC_API const char* mac_last_error(void);

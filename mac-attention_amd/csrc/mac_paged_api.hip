@@ -1,0 +1,190 @@
+// mac_paged_api.hip -- entry points of the paged chunk attention: argument
+// checks, the choice of the kernel body and of the stream form, the workspace.
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "mac_paged_attention.h"
+
+namespace mac {
+int fail(int code, const char* fmt, ...);
+}  // namespace mac
+
+namespace {
+
+using namespace mac;
+
+#define REQUIRE(cond, ...) \
+  do {                     \
+    if (!(cond)) return mac::fail(MAC_ERR_INVALID_ARGUMENT, __VA_ARGS__); \
+  } while (0)
+
+bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
+
+constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
+
+struct Choice {
+  int body = 0, cols = 0, task_rows = 0, unit_shift = 0, stream = 0, grid = 0;
+  size_t plan_bytes = 0, ml_bytes = 0, o_bytes = 0;
+  size_t bytes() const { return plan_bytes + ml_bytes + o_bytes; }
+};
+
+struct Variant {
+  int (*resident)(int, int, int);
+  hipError_t (*launch)(const PagedParams&, int, int, int, hipStream_t);
+};
+
+Variant variant(int q_dtype, int cache_dtype) {
+  if (q_dtype == MAC_DTYPE_BF16)
+    return cache_dtype == MAC_DTYPE_E4M3 ? Variant{paged_resident_bf16_fp8, paged_launch_bf16_fp8}
+                                         : Variant{paged_resident_bf16, paged_launch_bf16};
+  return cache_dtype == MAC_DTYPE_E4M3 ? Variant{paged_resident_f16_fp8, paged_launch_f16_fp8}
+                                       : Variant{paged_resident_f16, paged_launch_f16};
+}
+
+size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+
+// Body, task size and form for a call's shapes; false: too large.
+bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B, int64_t max_keys, Choice& ch) {
+  const int G = Hq / c.Hkv;
+  const int64_t cols = (total_q + B - 1) / B * G;  // columns of a request of average length
+  ch.body = cols <= 16 ? kBodyStream16 : (cols <= 32 ? kBodyStream32 : (cols <= 64 ? kBodyTile64 : kBodyTile128));
+  const int room = kBodyCols[ch.body];
+  ch.cols = G <= room ? room / G * G : room;  // whole rows where a row's heads fit
+  ch.task_rows = G <= room ? ch.cols / G : 2;
+  // bounds on the tasks: of this batch's rows, and of any row offsets (a
+  // request's rows lie within total_q)
+  const int64_t tasks = (std::min<int64_t>(total_q, total_q * G / ch.cols + B)) * c.Hkv;
+  const int64_t worst = static_cast<int64_t>(B) * ((total_q * G + ch.cols - 1) / ch.cols) * c.Hkv;
+  if (worst >= INT_MAX) return false;
+  const int resident = variant(q_dtype, c.cache_dtype).resident(c.D, ch.body, B);
+  ch.stream = ch.body <= kBodyStream32 || tasks < 2 * static_cast<int64_t>(resident);
+  ch.grid = resident;
+  if (!ch.stream) {
+    ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));
+    return true;
+  }
+  ch.unit_shift = 7;
+  while (ch.unit_shift < 30 && (((max_keys + (int64_t{1} << ch.unit_shift) - 1) >> ch.unit_shift) + 1) * worst >= INT_MAX) ++ch.unit_shift;
+  if (2 * worst >= INT_MAX || total_q * Hq > INT_MAX) return false;
+  ch.plan_bytes = up16(sizeof(int) * (static_cast<size_t>(B) + 1));
+  const size_t slots = 2 * static_cast<size_t>(ch.grid) * room;
+  ch.ml_bytes = slots * 2 * sizeof(float);
+  ch.o_bytes = slots * c.D * sizeof(float);
+  return true;
+}
+
+int check(const MacPagedCache* c, const MacPagedAttentionArgs* a) {
+  REQUIRE(c != nullptr && a != nullptr, "cache / args is NULL");
+  REQUIRE(c->struct_size == sizeof(MacPagedCache), "struct_size mismatch (%u vs %zu)", c->struct_size, sizeof(MacPagedCache));
+  REQUIRE(a->struct_size == sizeof(MacPagedAttentionArgs), "struct_size mismatch (%u vs %zu)", a->struct_size,
+          sizeof(MacPagedAttentionArgs));
+  REQUIRE(c->abi_version == MAC_ABI_VERSION && a->abi_version == MAC_ABI_VERSION, "abi_version mismatch");
+  REQUIRE(a->q_dtype == MAC_DTYPE_BF16 || a->q_dtype == MAC_DTYPE_F16, "q must be bfloat16 or float16");
+  REQUIRE(c->cache_dtype == MAC_DTYPE_E4M3 || c->cache_dtype == a->q_dtype, "the cache must hold e4m3 codes or q's type");
+  REQUIRE(c->D == 64 || c->D == 128 || c->D == 256, "head_dim must be 64, 128 or 256 (got %d)", c->D);
+  REQUIRE(a->Hq > 0 && c->Hkv > 0 && a->Hq % c->Hkv == 0, "Hq must be a positive multiple of Hkv");
+  REQUIRE(a->B >= 0 && a->B <= kMaxB, "B must be in [0, %d] (got %d)", kMaxB, a->B);
+  REQUIRE(a->total_q >= 0 && a->total_q <= INT_MAX / a->Hq, "total_q too large");
+  REQUIRE(c->num_pages > 0 && c->num_pages <= INT_MAX, "num_pages must be positive (and fit 31 bits)");
+  REQUIRE(c->page_size > 0 && (c->page_size & (c->page_size - 1)) == 0, "page_size must be a power of two (got %d)",
+          c->page_size);
+  REQUIRE(a->table_rows >= 0 && a->table_cols >= 0 &&
+              static_cast<int64_t>(a->table_cols) * c->page_size < (int64_t{1} << 30),
+          "page_table must name fewer than 2^30 keys per request");
+  REQUIRE(a->sm_scale > 0 && std::isfinite(a->sm_scale), "sm_scale must be positive");
+  REQUIRE(a->logit_cap >= 0 && std::isfinite(a->logit_cap), "logit_cap must be >= 0");
+  REQUIRE(c->k_scale > 0 && std::isfinite(c->k_scale) && c->v_scale > 0 && std::isfinite(c->v_scale),
+          "k_scale and v_scale must be positive");
+  if (c->kv_scales != nullptr) {
+    REQUIRE(c->cache_dtype == MAC_DTYPE_E4M3, "kv_scales belong to an e4m3 cache");
+    REQUIRE(c->k_scale == 1.0f && c->v_scale == 1.0f, "a row-scaled cache takes no k_scale / v_scale");
+    REQUIRE((reinterpret_cast<uintptr_t>(c->kv_scales) & 1) == 0, "kv_scales must be 2-byte aligned");
+  }
+  return MAC_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t mac_paged_chunk_attention_workspace(const MacPagedCache* c, const MacPagedAttentionArgs* a) {
+  if (check(c, a) != MAC_OK) return -1;
+  if (a->B == 0 || a->total_q == 0) return 0;
+  Choice ch;
+  if (!choose(*c, a->q_dtype, a->Hq, a->total_q, a->B, static_cast<int64_t>(a->table_cols) * c->page_size, ch)) return 0;
+  return static_cast<int64_t>(ch.bytes());
+}
+
+extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedAttentionArgs* a, void* workspace,
+                                         int64_t workspace_bytes, void* stream) {
+  if (int rc = check(c, a)) return rc;
+  if (a->B == 0 || a->total_q == 0) return MAC_OK;
+  REQUIRE(a->q && c->k_cache && c->v_cache && a->qo_indptr && a->kv_lens && a->out && a->out_lse, "null pointer argument");
+  REQUIRE(a->page_table || a->table_cols == 0 || a->table_rows == 0, "null pointer argument");
+  REQUIRE(aligned16(a->q) && ((a->q_stride0 | a->q_stride1) & 7) == 0, "q rows must be 16-byte aligned");
+  REQUIRE(aligned16(c->k_cache) && aligned16(c->v_cache), "k_cache and v_cache must be 16-byte aligned");
+  REQUIRE(((c->k_page_stride | c->k_slot_stride | c->k_head_stride | c->v_page_stride | c->v_slot_stride |
+            c->v_head_stride) & 15) == 0,
+          "cache strides must be multiples of 16 bytes");
+  REQUIRE(aligned16(a->out), "out must be 16-byte aligned");
+  Choice ch;
+  REQUIRE(choose(*c, a->q_dtype, a->Hq, a->total_q, a->B, static_cast<int64_t>(a->table_cols) * c->page_size, ch),
+          "batch too large");
+  REQUIRE(aligned16(workspace) && workspace_bytes >= static_cast<int64_t>(ch.bytes()) && (workspace || ch.bytes() == 0),
+          "workspace too small or misaligned (needs %zu bytes)", ch.bytes());
+  const int G = a->Hq / c->Hkv;
+  const double log2e = 1.4426950408889634;
+  PagedParams p{};
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.k = static_cast<const char*>(c->k_cache);
+  p.v = static_cast<const char*>(c->v_cache);
+  p.scales = static_cast<const uint16_t*>(c->kv_scales);
+  p.qo_indptr = a->qo_indptr;
+  p.kv_lens = a->kv_lens;
+  p.table = a->page_table;
+  p.req_ids = a->req_ids;
+  p.out = static_cast<uint16_t*>(a->out);
+  p.lse = a->out_lse;
+  if (ch.stream) {
+    char* w = static_cast<char*>(workspace);
+    p.plan = reinterpret_cast<int32_t*>(w);
+    p.part_ml = reinterpret_cast<float*>(w + ch.plan_bytes);
+    p.part_o = reinterpret_cast<float*>(w + ch.plan_bytes + ch.ml_bytes);
+  }
+  p.q_ts = a->q_stride0;
+  p.q_hs = a->q_stride1;
+  p.k_ps = c->k_page_stride;
+  p.k_ss = c->k_slot_stride;
+  p.k_hs = c->k_head_stride;
+  p.v_ps = c->v_page_stride;
+  p.v_ss = c->v_slot_stride;
+  p.v_hs = c->v_head_stride;
+  p.table_stride = a->table_stride;
+  p.total_q = a->total_q;
+  p.num_pages = c->num_pages;
+  p.B = a->B;
+  p.Hq = a->Hq;
+  p.Hkv = c->Hkv;
+  p.G = G;
+  p.table_rows = a->table_rows;
+  p.table_cols = a->table_cols;
+  p.page_shift = __builtin_ctz(c->page_size);
+  // (a window of 2^30 keys or more covers any request's)
+  p.window_left = a->window_left < 0 || a->window_left >= (1 << 30) ? -1 : a->window_left;
+  p.cols = ch.cols;
+  p.task_rows = ch.task_rows;
+  p.unit_shift = ch.unit_shift;
+  p.stream = ch.stream;
+  p.grid = ch.grid;
+  p.min_units = 1;
+  const double raw = a->sm_scale * c->k_scale;
+  p.q_scale = static_cast<float>(a->logit_cap > 0 ? 1.0 : raw * log2e);
+  p.cap_in = a->logit_cap > 0 ? static_cast<float>(2.0 * log2e * raw / a->logit_cap) : 0.0f;
+  p.cap_out = static_cast<float>(a->logit_cap * log2e);
+  p.v_scale = c->v_scale;
+  const hipError_t e = variant(a->q_dtype, c->cache_dtype).launch(p, c->D, ch.body, ch.grid, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return mac::fail(MAC_ERR_HIP, "paged chunk attention: %s", hipGetErrorString(e));
+  return MAC_OK;
+}

@@ -1,0 +1,250 @@
+// mac_paged_attention.h -- parameters, planning and element types shared by
+// the paged chunk attention's entry point and kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "mac_attention_amd.h"
+#include "mac_common.h"
+
+namespace mac {
+
+// What the kernels read.  A call's queries are cut into tasks of `cols`
+// (row, head) columns of one request and KV head; stream form: the tasks' keys
+// laid end to end in units of 2^unit_shift keys, dealt to the workgroups in
+// equal runs.
+struct PagedParams {
+  const uint16_t* q;
+  const char* k;
+  const char* v;
+  const uint16_t* scales;  // [pages, Hkv, P] (K byte low, V byte high), or NULL
+  const int32_t* qo_indptr;
+  const int32_t* kv_lens;
+  const int32_t* table;
+  const int32_t* req_ids;  // row of the table for each request, or NULL: the request's number
+  uint16_t* out;
+  float* lse;
+  float* part_o;   // stream form: [2 grid][cols][D] unnormalised partial outputs
+  float* part_ml;  // [2 grid][cols][2] their reference points (log2 units) and sums
+  int32_t* plan;   // [B + 1] units before each request, for the combining launch
+  int64_t q_ts, q_hs;                          // elements
+  int64_t k_ps, k_ss, k_hs, v_ps, v_ss, v_hs;  // bytes
+  int64_t table_stride;
+  int64_t total_q;
+  int64_t num_pages;
+  int B, Hq, Hkv, G;
+  int table_rows, table_cols, page_shift;
+  int window_left;  // < 0: none
+  int cols;         // columns of a task (whole rows where a row's heads fit one)
+  int task_rows;    // most rows that a task's columns touch
+  int unit_shift;   // stream form; 0 units: plain form
+  int stream;       // 1: stream form
+  int grid;         // workgroups of the stream form (slots hold 2 partials of each)
+  int min_units;    // least units per workgroup worth starting it for
+  float q_scale;    // sm_scale k_scale log2(e); with a cap: 1 (scores are capped to log2 units)
+  float cap_in, cap_out;  // 2 log2(e) sm_scale k_scale / cap, cap log2(e); 0: no cap
+  float v_scale;
+};
+
+// A request's rows, keys and tasks; all 0 for one whose rows do not lie in the
+// buffers.
+struct PagedRequest {
+  int q0, n;    // first row, rows
+  int len;      // kv length (row r sits at position len - n + r)
+  int keys;     // cached keys that the table can name
+  int tasks;    // column tasks per KV head
+  int units;    // stream form: units per task
+};
+
+__device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int b) {
+  PagedRequest r;
+  r.q0 = p.qo_indptr[b];
+  const int q1 = p.qo_indptr[b + 1];
+  r.len = max(p.kv_lens[b], 0);
+  const int row = p.req_ids != nullptr ? p.req_ids[b] : b;
+  r.n = r.q0 >= 0 && q1 > r.q0 && q1 <= p.total_q ? q1 - r.q0 : 0;
+  // (the table holds fewer than 2^30 keys a request, checked on the host)
+  r.keys = row >= 0 && row < p.table_rows ? min(r.len, p.table_cols << p.page_shift) : 0;
+  r.tasks = static_cast<int>((static_cast<int64_t>(r.n) * p.G + p.cols - 1) / p.cols);
+  const int span = p.window_left < 0 ? r.keys : min(r.keys, p.window_left + p.task_rows);
+  r.units = max((span + (1 << p.unit_shift) - 1) >> p.unit_shift, 1);
+  return r;
+}
+
+// Units (stream form) or tasks (plain form) of a request.
+__device__ __forceinline__ int paged_weight(const PagedParams& p, const PagedRequest& r) {
+  return r.tasks * p.Hkv * (p.stream ? r.units : 1);
+}
+
+// Exclusive prefix of the requests' weights in s_pre[B + 1], by a workgroup of
+// 256 threads; ends with a barrier.  s_tmp: 4 entries.
+__device__ __forceinline__ void paged_plan(const PagedParams& p, int* s_pre, int* s_tmp) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = ceil_div(p.B, 256);
+  const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+  int sum = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int w = paged_weight(p, paged_request(p, b));
+    s_pre[b] = w;
+    sum += w;
+  }
+  int x = sum;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int y = __shfl_up(x, off);
+    if (lane >= off) x += y;
+  }
+  if (lane == 63) s_tmp[wave] = x;
+  __syncthreads();
+  int acc = x - sum, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) acc += s_tmp[w];
+    total += s_tmp[w];
+  }
+  for (int b = b0; b < b1; ++b) {
+    const int w = s_pre[b];
+    s_pre[b] = acc;
+    acc += w;
+  }
+  if (tid == 0) s_pre[p.B] = total;
+  __syncthreads();
+}
+
+// Largest b < B with pre[b] <= x.
+__device__ __forceinline__ int paged_find(const int* s_pre, int B, int x) {
+  int lo = 0, hi = B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_pre[mid] <= x) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Stream form: workgroups that get units, and the first unit of workgroup w.
+__device__ __forceinline__ int stream_groups(const PagedParams& p, int total) {
+  return min(p.grid, max(total / p.min_units, 1));
+}
+__device__ __forceinline__ int stream_begin(int w, int total, int groups) {
+  return static_cast<int>(static_cast<int64_t>(w) * total / groups);
+}
+// The workgroup whose run holds unit x.
+__device__ __forceinline__ int stream_owner(int x, int total, int groups) {
+  return static_cast<int>((static_cast<int64_t>(x + 1) * groups + total - 1) / total) - 1;
+}
+
+// One of a task's runs of keys.
+struct PagedTask {
+  int b, hkv, gc0;      // request, KV head, first column of the request's rows x G
+  int q0, n, len;       // of the request
+  int nc;               // columns
+  int row0, row1;       // first and last row
+  int klo, khi;         // keys to attend over in this run
+  const int32_t* table;
+};
+
+__device__ __forceinline__ PagedTask paged_task(const PagedParams& p, int b, const PagedRequest& r, int index) {
+  PagedTask t;
+  t.b = b;
+  t.hkv = index / r.tasks;
+  const int ct = index - t.hkv * r.tasks;
+  t.q0 = r.q0;
+  t.n = r.n;
+  t.len = r.len;
+  // (columns of a request fit 31 bits, checked on the host)
+  t.gc0 = ct * p.cols;
+  t.nc = min(p.cols, r.n * p.G - t.gc0);
+  t.row0 = t.gc0 / p.G;
+  t.row1 = (t.gc0 + t.nc - 1) / p.G;
+  const int first = r.len - r.n + t.row0, last = r.len - r.n + t.row1;
+  t.klo = p.window_left < 0 ? 0 : max(first - p.window_left, 0);
+  t.khi = min(max(last + 1, 0), r.keys);
+  const int row = p.req_ids != nullptr ? p.req_ids[b] : b;
+  t.table = p.table + static_cast<int64_t>(row < 0 || row >= p.table_rows ? 0 : row) * p.table_stride;
+  return t;
+}
+
+// 16-bit element types.
+typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 pa_f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 pa_f16x8 __attribute__((ext_vector_type(8)));
+typedef float pa_f32x4 __attribute__((ext_vector_type(4)));
+
+template <int kT>
+struct PagedElem;
+
+template <>
+struct PagedElem<MAC_DTYPE_BF16> {
+  static __device__ __forceinline__ pa_f32x4 mfma(const uint4& a, const uint4& b, pa_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a), __builtin_bit_cast(pa_bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const pa_bf16x2 v = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  // two codes (the low or the high half of w) times the power of two s: exact
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t decode2(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, kHigh));
+  }
+  static __device__ __forceinline__ float low(uint32_t w) { return bf16_lo(w); }
+  static __device__ __forceinline__ float high(uint32_t w) { return bf16_hi(w); }
+  static __device__ __forceinline__ bool not_finite(uint32_t w) {
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  }
+};
+
+template <>
+struct PagedElem<MAC_DTYPE_F16> {
+  static __device__ __forceinline__ pa_f32x4 mfma(const uint4& a, const uint4& b, pa_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_f16x8, a), __builtin_bit_cast(pa_f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const pa_f16x2 v = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+  template <bool kHigh>
+  static __device__ __forceinline__ uint32_t decode2(uint32_t w, float s) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, kHigh));
+  }
+  static __device__ __forceinline__ float low(uint32_t w) { return static_cast<float>(__builtin_bit_cast(pa_f16x2, w)[0]); }
+  static __device__ __forceinline__ float high(uint32_t w) { return static_cast<float>(__builtin_bit_cast(pa_f16x2, w)[1]); }
+  static __device__ __forceinline__ bool not_finite(uint32_t w) {
+    return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u;
+  }
+};
+
+// Sixteen codes as two vectors of eight 16-bit values.
+template <int kT>
+__device__ __forceinline__ void decode16(const uint4& w, float s, uint4& a, uint4& b) {
+  typedef PagedElem<kT> E;
+  a = make_uint4(E::template decode2<false>(w.x, s), E::template decode2<true>(w.x, s),
+                 E::template decode2<false>(w.y, s), E::template decode2<true>(w.y, s));
+  b = make_uint4(E::template decode2<false>(w.z, s), E::template decode2<true>(w.z, s),
+                 E::template decode2<false>(w.w, s), E::template decode2<true>(w.w, s));
+}
+template <int kT>
+__device__ __forceinline__ bool not_finite(const uint4& w) {
+  typedef PagedElem<kT> E;
+  return E::not_finite(w.x) || E::not_finite(w.y) || E::not_finite(w.z) || E::not_finite(w.w);
+}
+
+// Host: launch of one variant (mac_paged_attention.hip is compiled once for
+// each of them).
+enum { kBodyStream16 = 0, kBodyStream32 = 1, kBodyTile64 = 2, kBodyTile128 = 3, kBodies = 4 };
+constexpr int kBodyCols[kBodies] = {16, 32, 64, 128};
+
+// Resident workgroups of a body on the current device, and its launch (with
+// the combining one in the stream form).
+#define MAC_PAGED_VARIANT_DECL(name)                                                       \
+  int paged_resident_##name(int D, int body, int B);                                       \
+  hipError_t paged_launch_##name(const PagedParams& p, int D, int body, int grid, hipStream_t stream);
+MAC_PAGED_VARIANT_DECL(bf16)
+MAC_PAGED_VARIANT_DECL(f16)
+MAC_PAGED_VARIANT_DECL(bf16_fp8)
+MAC_PAGED_VARIANT_DECL(f16_fp8)
+
+}  // namespace mac

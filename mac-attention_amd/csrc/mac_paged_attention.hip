@@ -1,0 +1,874 @@
+// mac_paged_attention.hip -- attention of a chunk of new tokens over a paged
+// K/V cache for MI355X (gfx950).  Compiled once per variant (queries bf16 or
+// fp16; cache of the same type or e4m3): MAC_PAGED_T, MAC_PAGED_F8 and
+// MAC_PAGED_NAME come from the build.
+//
+// Row r of a request with n new rows and a cache of len keys sits at position
+// len - n + r and attends to the keys [max(pos - window, 0), pos]:
+//   s_k = q . k_k sm_scale     (or cap tanh(q . k_k sm_scale / cap))
+//   out = sum_k e^(s_k - m) v_k / l,  lse = m + log l,  l = sum_k e^(s_k - m)
+// in one pass over the keys with a running reference point m and sum l in fp32.
+//
+// Columns.  A GQA group's heads share their keys, so the (row, head) pairs of a
+// request and KV head are the columns of S^T = K Q^T and O^T += V^T P^T on
+// v_mfma_f32_16x16x32: 16 consecutive columns a tile, whatever the group size
+// (one token of 4 heads, five drafted tokens of 8, a chunk's rows).  The lane
+// (quad, col) = (lane / 16, lane % 16) holds column col: its scores of keys 16 t
+// + 4 quad + (0..3), and of the output dims 16 dt + 4 quad + (0..3).
+//
+// 8-bit rows become 16-bit values when they are staged: every e4m3 value times
+// a power of two is exact in bf16, and gfx950 converts two codes and applies
+// the row's scale in one instruction, so the products run as for 16-bit rows.
+// A static k_scale is part of the softmax scale, v_scale of the final
+// normalisation.  P is rounded to the queries' type for its product (2^-9 or
+// 2^-12 of each weight, as much as the output's own rounding); sums are fp32.
+//
+// Masked keys: keys past a row's range, past the cache or without a page get
+// s = -inf, and V of keys that no row may see is zeroed when staged.  A key that
+// some rows see and others do not is left in place: where such a block holds V
+// that is not finite (0 x NaN), its P V is summed without the masked keys
+// (pv_exact).
+
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "mac_paged_attention.h"
+
+namespace {
+
+using namespace mac;
+
+constexpr int kT = MAC_PAGED_T;
+constexpr bool kF8 = MAC_PAGED_F8;
+typedef PagedElem<kT> E;
+typedef pa_f32x4 f32x4;
+
+// Four dims of V, one row each of four: the transposing LDS read (lds_read_tr16)
+// of 16-bit elements of either type.
+__device__ __forceinline__ uint2 read_tr(const uint16_t* at) { return __builtin_bit_cast(uint2, lds_read_tr16(at)); }
+__device__ __forceinline__ uint4 join(const uint2& a, const uint2& b) { return make_uint4(a.x, a.y, b.x, b.y); }
+
+// Softmax state of one column tile: raw-score reference point m (-inf: no key
+// seen), the scaled score past which it moves, the lane's part of the sum, and
+// whether a reference point of the wave is so large that m scale, rounded on its
+// own, would be off by whole powers of two (then (s - m) scale is formed instead
+// of one fma: 2^20 leaves 2^-4 of one).
+struct Column {
+  float m, past, l;
+  bool far;
+};
+__device__ __forceinline__ Column fresh_column() { return Column{-INFINITY, -INFINITY, 0.0f, false}; }
+constexpr float kFar = 1048576.0f;
+
+// Scores of 32 keys (c[t][r]: key 16 t + 4 quad + r) to weights in f[8], moving
+// the reference point where a score exceeds it by 2^8 (lazily: p <= 2^8 is as
+// exact, and most blocks rescale nothing).  Called by whole waves.
+template <int kDT>
+__device__ __forceinline__ void weigh(const f32x4 (&c)[2], float scale, Column& s, f32x4 (&acc)[kDT], float (&f)[8]) {
+  const float sv[8] = {c[0][0], c[0][1], c[0][2], c[0][3], c[1][0], c[1][1], c[1][2], c[1][3]};
+  const float top = max8_nonan(sv);
+  if (__any(top * scale > s.past)) {
+    const float bm = quad_max(top);
+    const float m_new = max3_nonan(s.m, bm, bm);
+    const float alpha = s.m == m_new ? 1.0f : fast_exp2((s.m - m_new) * scale);
+    s.m = m_new;
+    s.past = m_new * scale + 8.0f;
+    s.far = __any(fabsf(m_new) * scale > kFar && m_new != -INFINITY);
+    s.l *= alpha;
+#pragma unroll
+    for (int dt = 0; dt < kDT; ++dt) acc[dt] *= alpha;
+  }
+  const float mo = s.m == -INFINITY ? 0.0f : -s.m * scale;
+  float sum = 0.0f;
+  if (s.far) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fast_exp2((s.m == -INFINITY ? sv[e] : sv[e] - s.m) * scale);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fast_exp2(fmaf(sv[e], scale, mo));
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sum += f[e];
+  s.l += sum;
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(E::pack2(f[0], f[1]), E::pack2(f[2], f[3]), E::pack2(f[4], f[5]), E::pack2(f[6], f[7]));
+}
+
+// Logit cap: raw scores to capped ones in log2 units, cap log2(e) tanh(x) with
+// tanh(x) = 1 - 2 / (1 + e^2x) (off by 2^-23 of the cap: the scores are fp32).
+__device__ __forceinline__ void cap_scores(f32x4 (&c)[2], float cap_in, float cap_out) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      c[t][r] = cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(c[t][r] * cap_in)));
+}
+
+// The keys of 32 from `base` that a row with the range [lo, hi) sees, less
+// `bad`, as bits of the lane's own keys: bit 16 t + r.
+__device__ __forceinline__ uint32_t seen_keys(int base, int lo, int hi, uint32_t bad, int quad) {
+  const int a = min(max(lo - base, 0), 32), z = min(max(hi - base, 0), 32);
+  const uint64_t range = ((1ull << z) - 1) & ~((1ull << a) - 1);
+  return (static_cast<uint32_t>(range) & ~bad) >> (4 * quad);
+}
+__device__ __forceinline__ void mask_scores(f32x4 (&c)[2], uint32_t seen) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) c[t][r] = (seen >> (16 * t + r)) & 1 ? c[t][r] : -INFINITY;
+}
+
+// O^T += V^T P^T of 32 keys without the masked ones, on the vector units: v
+// points at the block's first row (row_units 16-byte units apart).
+template <int kDT>
+__device__ __forceinline__ void pv_exact(f32x4 (&acc)[kDT], const float (&f)[8], uint32_t seen, const uint16_t* v,
+                                                   int row_halves, int quad, int col) {
+  float g[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] = (seen >> (16 * (e >> 2) + (e & 3))) & 1 ? f[e] : -1.0f;
+#pragma unroll 1
+  for (int kq = 0; kq < 4; ++kq) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float w = __shfl(g[e], 16 * kq + col);
+      const uint16_t* row = v + (16 * (e >> 2) + 4 * kq + (e & 3)) * row_halves + 4 * quad;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        const uint2 x = *reinterpret_cast<const uint2*>(row + 16 * dt);
+        if (w >= 0.0f || w != w) {
+          acc[dt][0] += w * E::low(x.x);
+          acc[dt][1] += w * E::high(x.x);
+          acc[dt][2] += w * E::low(x.y);
+          acc[dt][3] += w * E::high(x.y);
+        }
+      }
+    }
+  }
+}
+
+// The rows and columns of one run as a lane sees them.
+struct LaneColumn {
+  int row, head;  // in the request, in the group
+  bool ok;
+  int lo, hi;  // keys the row sees
+};
+__device__ __forceinline__ LaneColumn lane_column(const PagedParams& p, const PagedTask& t, int c) {
+  LaneColumn k;
+  k.ok = c < t.nc;
+  const int gc = t.gc0 + min(c, t.nc - 1);  // (a column past the task computes its last one and stores nothing)
+  k.row = gc / p.G;
+  k.head = gc - k.row * p.G;
+  const int pos = t.len - t.n + k.row;
+  k.lo = p.window_left < 0 ? 0 : max(pos - p.window_left, 0);
+  k.hi = pos + 1;
+  return k;
+}
+
+// One run's place in the stream or in the task list.
+struct Run {
+  PagedTask task;
+  bool whole;  // the task's keys are all here: results go straight out
+  int slot;    // else the partial state's place
+};
+
+// Run `i` of this workgroup.  Stream form: x is the unit it starts at (moved
+// past the run); plain form: the task number.  False: no more.
+__device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre, int x0, int x1, int& x, Run& r) {
+  if (x >= x1) return false;
+  const int b = __builtin_amdgcn_readfirstlane(paged_find(s_pre, p.B, x));
+  const PagedRequest q = paged_request(p, b);
+  const int at = x - s_pre[b];
+  if (!p.stream) {
+    // longest rows first within a request, its KV heads side by side
+    const int index = at / p.Hkv, h = at - index * p.Hkv;
+    r.task = paged_task(p, b, q, h * q.tasks + (q.tasks - 1 - index));
+    r.whole = true;
+    r.slot = 0;
+    x += gridDim.x;
+    return true;
+  }
+  const int index = at / q.units, unit = at - index * q.units;
+  const int end = min(x1, x + q.units - unit);
+  r.task = paged_task(p, b, q, index);
+  r.whole = unit == 0 && end - x == q.units;
+  r.slot = 2 * static_cast<int>(blockIdx.x) + (x == x0 ? 0 : 1);
+  const int lo = r.task.klo + static_cast<int>(min(static_cast<int64_t>(unit) << p.unit_shift, int64_t{1} << 30));
+  const int hi = r.task.klo + static_cast<int>(min(static_cast<int64_t>(unit + end - x) << p.unit_shift, int64_t{1} << 30));
+  r.task.klo = min(lo, r.task.khi);
+  r.task.khi = min(hi, r.task.khi);
+  x = end;
+  return true;
+}
+
+// ------------------------------------------------------------ stream body ---
+
+// Few columns (16 kPer): the bytes of K and V bound the call, so the four waves
+// take different keys, 32 at a time, and meet once, at the end of a run.  A
+// wave needs no barrier on its way: K goes from memory straight into the
+// matrix operand's registers (lane (quad, col) loads key col, 16-byte chunks
+// quad + 4 c), V through a tile of LDS of its own, which transposes it.  Two
+// blocks' registers: one computes while the other is in flight, and the page
+// entries go out a block ahead of the rows that need them.
+template <int D, int kPer>
+__global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
+  constexpr int kS = D / 32;                  // k-steps of a score
+  constexpr int kCh = kF8 ? D / 64 : D / 32;  // 16-byte chunks of a row per lane
+  constexpr int kVU = D / 8 + 2;              // 16-byte units per staged V row
+  constexpr int kDT = D / 16;
+  constexpr int kC = 16 * kPer;
+  constexpr int kOut = D + 4;                 // floats per column of the joined state
+  extern __shared__ int s_pre[];
+  __shared__ int s_tmp[4];
+  __shared__ uint4 s_v[4][32 * kVU];
+  __shared__ float s_m[4][kC], s_l[4][kC];
+  static_assert(16 * kOut * 4 <= 32 * kVU * 16, "a wave's state fits its V tile");
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
+  paged_plan(p, s_pre, s_tmp);
+  const int total = s_pre[p.B];
+  const int groups = stream_groups(p, total);
+  if (blockIdx.x == 0)
+    for (int b = tid; b <= p.B; b += 256) p.plan[b] = s_pre[b];
+  if (static_cast<int>(blockIdx.x) >= groups) return;
+  const int x0 = stream_begin(blockIdx.x, total, groups), x1 = stream_begin(blockIdx.x + 1, total, groups);
+
+  const float scale = p.q_scale;
+  const bool scaled = kF8 && p.scales != nullptr;
+  const int slot_mask = (1 << p.page_shift) - 1;
+  uint4* const vw = &s_v[wave][0] + col * kVU + (kF8 ? 2 * quad : quad);
+  const uint16_t* const vr = reinterpret_cast<const uint16_t*>(&s_v[wave][0]) + (4 * quad + (col >> 2)) * (kVU * 8) + 4 * (col & 3);
+
+  struct Block {
+    uint4 k[2][kCh], v[2][kCh];
+    uint32_t sc[2];
+    uint32_t bad;  // keys of the 32 without a row
+  };
+
+  int x = x0;
+  Run run;
+  while (next_run(p, s_pre, x0, x1, x, run)) {
+    const PagedTask& t = run.task;
+    // the wave's columns
+    LaneColumn lc[kPer];
+    uint4 q[kPer][kS];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      lc[c] = lane_column(p, t, 16 * c + col);
+      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
+#pragma unroll
+      for (int s = 0; s < kS; ++s)
+        q[c][s] = *reinterpret_cast<const uint4*>(at + (kF8 ? 64 * (s >> 1) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad));
+    }
+    // keys that every row of the task sees
+    const int all_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
+    const int all_hi = t.len - t.n + t.row0 + 1;
+
+    const char* const kb = p.k + t.hkv * p.k_hs + 16 * quad;
+    const char* const vb = p.v + t.hkv * p.v_hs + 16 * quad;
+    const int last_entry = p.table_cols - 1;
+    auto entries = [&](int base, int (&e)[2]) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) e[i] = t.table[min((base + 16 * i + col) >> p.page_shift, last_entry)];
+    };
+    auto load = [&](int base, const int (&e)[2], Block& blk) {
+      uint32_t have = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = base + 16 * i + col;
+        const bool ok = key < t.khi && e[i] >= 0 && e[i] < p.num_pages;
+        have |= static_cast<uint32_t>(__ballot(ok) & 0xffffu) << (16 * i);
+        const int64_t page = ok ? e[i] : 0;
+        const int slot = ok ? key & slot_mask : 0;
+        const char* ka = kb + page * p.k_ps + slot * p.k_ss;
+        const char* va = vb + page * p.v_ps + slot * p.v_ss;
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) {
+          blk.k[i][c] = *reinterpret_cast<const uint4*>(ka + 64 * c);
+          blk.v[i][c] = *reinterpret_cast<const uint4*>(va + 64 * c);
+        }
+        if (scaled) blk.sc[i] = p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot];
+      }
+      blk.bad = ~have;
+    };
+
+    Column st[kPer];
+    f32x4 acc[kPer][kDT];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      st[c] = fresh_column();
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) acc[c][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    auto compute = [&](int base, const Block& blk) {
+      const uint32_t bad = __builtin_amdgcn_readfirstlane(blk.bad);
+      const bool masked = base < all_lo || base + 32 > all_hi || bad != 0;
+      float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
+      if (scaled) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          ks[i] = __uint_as_float((blk.sc[i] & 255u) << 23);
+          vs[i] = __uint_as_float((blk.sc[i] >> 8) << 23);
+        }
+      }
+      // V to LDS
+      bool odd = false;
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the block before is read)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const bool ok = !((bad >> (16 * i + col)) & 1);
+#pragma unroll
+        for (int c = 0; c < kCh; ++c) {
+          uint4 w[2];
+          if constexpr (kF8) decode16<kT>(blk.v[i][c], vs[i], w[0], w[1]);
+          else w[0] = blk.v[i][c];
+#pragma unroll
+          for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
+            if (masked) {
+              if (!ok) w[h] = make_uint4(0, 0, 0, 0);
+              odd = odd || not_finite<kT>(w[h]);
+            }
+            vw[16 * i * kVU + (kF8 ? 8 : 4) * c + h] = w[h];
+          }
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      // scores
+      f32x4 s4[kPer][2];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) s4[c][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int ch = 0; ch < kCh; ++ch) {
+        uint4 a[2][2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if constexpr (kF8) decode16<kT>(blk.k[i][ch], ks[i], a[i][0], a[i][1]);
+          else a[i][0] = blk.k[i][ch];
+        }
+#pragma unroll
+        for (int h = 0; h < (kF8 ? 2 : 1); ++h)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a[i][h], q[c][(kF8 ? 2 : 1) * ch + h], s4[c][i]);
+      }
+      float f[kPer][8];
+      uint32_t seen[kPer];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) {
+        if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
+        seen[c] = 0xffffffffu;
+        if (masked) {
+          seen[c] = seen_keys(base, lc[c].lo, min(lc[c].hi, t.khi), bad, quad);
+          mask_scores(s4[c], seen[c]);
+        }
+        weigh(s4[c], scale, st[c], acc[c], f[c]);
+      }
+      if (masked && __any(odd)) {
+#pragma unroll
+        for (int c = 0; c < kPer; ++c)
+          pv_exact(acc[c], f[c], seen[c], reinterpret_cast<const uint16_t*>(&s_v[wave][0]), kVU * 8, quad, col);
+        return;
+      }
+      uint4 pb[kPer];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) {
+        const uint4 a = join(read_tr(vr + 16 * dt), read_tr(vr + 16 * kVU * 8 + 16 * dt));
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
+      }
+    };
+
+    // the wave's blocks: every fourth of the run's
+    Block ba, bb;
+    int ea[2], eb[2];
+    int base = t.klo + 32 * wave;
+    if (base < t.khi) {
+      entries(base, ea);
+      entries(base + 128, eb);
+      load(base, ea, ba);
+      while (true) {
+        if (base + 128 < t.khi) {
+          entries(base + 256, ea);
+          __builtin_amdgcn_sched_barrier(0);
+          load(base + 128, eb, bb);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        compute(base, ba);
+        base += 128;
+        if (base >= t.khi) break;
+        if (base + 128 < t.khi) {
+          entries(base + 256, eb);
+          __builtin_amdgcn_sched_barrier(0);
+          load(base + 128, ea, ba);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        compute(base, bb);
+        base += 128;
+        if (base >= t.khi) break;
+      }
+    }
+
+    // the four waves' states joined
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      const float l = quad_sum(st[c].l);
+      if (quad == 0) {
+        s_m[wave][16 * c + col] = st[c].m * scale;  // (-inf: no key)
+        s_l[wave][16 * c + col] = l;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      float m = s_m[0][16 * c + col];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][16 * c + col]);
+      const float own = s_m[wave][16 * c + col];
+      // (-inf for a state without keys: weight 0, or 1 where no wave has any)
+      const float f = own == m ? 1.0f : fast_exp2(own - m);
+      float* o = reinterpret_cast<float*>(&s_v[wave][0]) + col * kOut + 4 * quad;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[c][dt] * f;
+      __syncthreads();
+      // 16 threads per column, D / 16 dims each
+      const int cc = tid >> 4, d0 = (tid & 15) * kDT;
+      const int gcol = 16 * c + cc;
+      float mx = s_m[0][gcol], l = 0.0f;
+#pragma unroll
+      for (int w = 1; w < 4; ++w) mx = fmaxf(mx, s_m[w][gcol]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) l += s_l[w][gcol] * (s_m[w][gcol] == mx ? 1.0f : fast_exp2(s_m[w][gcol] - mx));
+      if (gcol < t.nc) {
+        float r[kDT];
+#pragma unroll
+        for (int i = 0; i < kDT; i += 4) {
+          f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&s_v[w][0]) + cc * kOut + d0 + i);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) r[i + j] = sum[j];
+        }
+        if (run.whole) {
+          const LaneColumn k = lane_column(p, t, gcol);
+          const int64_t at = static_cast<int64_t>(t.q0 + k.row) * p.Hq + t.hkv * p.G + k.head;
+          const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+#pragma unroll
+          for (int i = 0; i < kDT; i += 4)
+            *reinterpret_cast<uint2*>(p.out + at * D + d0 + i) =
+                make_uint2(E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv));
+          if (d0 == 0) p.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
+        } else {
+          const int64_t at = static_cast<int64_t>(run.slot) * kC + gcol;
+#pragma unroll
+          for (int i = 0; i < kDT; i += 4)
+            *reinterpret_cast<f32x4*>(p.part_o + at * D + d0 + i) = f32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+          if (d0 == 0) {
+            p.part_ml[at * 2] = mx;
+            p.part_ml[at * 2 + 1] = l;
+          }
+        }
+      }
+      __syncthreads();  // the tiles and sums are free again
+    }
+  }
+}
+
+// -------------------------------------------------------------- tile body ---
+
+// Many columns (64 kPer): the matrix cores bound the call, so the four waves
+// take different columns, kPer tiles each, and share K and V tiles of kBlk keys
+// in double-buffered LDS.  K chunk c (16 bytes) of key k lies at position c ^ (k
+// & 15) (& 7 for 64 dims) of its row, so that the 16 keys an operand reads lie
+// on different banks; V rows are padded by 32 bytes for the transposing reads.
+template <int D, int kPer, int kBlk, int kOcc>
+__global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
+  constexpr int kS = D / 32;
+  constexpr int kDT = D / 16;
+  constexpr int kKU = D / 8;               // 16-byte units per staged K row
+  constexpr int kVU = D / 8 + 2;
+  constexpr int kSwz = kKU < 16 ? kKU - 1 : 15;
+  constexpr int kRowCh = kF8 ? D / 16 : D / 8;  // 16-byte chunks of a cached row
+  constexpr int kStep = 256 / kRowCh;           // keys per pass of the workgroup
+  constexpr int kLd = kBlk / kStep;
+  constexpr int kSub = kBlk / 32;
+  static_assert(kLd >= 1, "a block is at least one pass");
+  extern __shared__ int s_pre[];
+  __shared__ int s_tmp[4];
+  __shared__ uint4 s_k[2][kBlk * kKU];
+  __shared__ uint4 s_v[2][kBlk * kVU];
+  __shared__ uint4 s_bad[2][kSub];  // per wave: its keys (of each 32) without a row
+  __shared__ uint4 s_odd[2];        // per wave: V that is not finite among its rows (looked for in masked blocks)
+
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
+  paged_plan(p, s_pre, s_tmp);
+  const int total = s_pre[p.B];
+  int x0 = blockIdx.x, x1 = total;
+  if (p.stream) {
+    const int groups = stream_groups(p, total);
+    if (blockIdx.x == 0)
+      for (int b = tid; b <= p.B; b += 256) p.plan[b] = s_pre[b];
+    if (static_cast<int>(blockIdx.x) >= groups) return;
+    x0 = stream_begin(blockIdx.x, total, groups);
+    x1 = stream_begin(blockIdx.x + 1, total, groups);
+  }
+  const float scale = p.q_scale;
+  const bool scaled = kF8 && p.scales != nullptr;
+  const int slot_mask = (1 << p.page_shift) - 1;
+  // loader: thread t stages chunk t % kRowCh of keys t / kRowCh + kStep i
+  const int ld_key = tid / kRowCh, ld_ch = tid % kRowCh;
+  // compute: the lane's V^T read position
+  const int rd_v = (4 * quad + (col >> 2)) * (kVU * 8) + 4 * (col & 3);
+
+  int x = x0;
+  Run run;
+  while (next_run(p, s_pre, x0, x1, x, run)) {
+    const PagedTask& t = run.task;
+    LaneColumn lc[kPer];
+    uint4 q[kPer][kS];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      lc[c] = lane_column(p, t, 16 * (kPer * wave + c) + col);
+      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
+#pragma unroll
+      for (int s = 0; s < kS; ++s) q[c][s] = *reinterpret_cast<const uint4*>(at + 32 * s + 8 * quad);
+    }
+    // the wave's first and last row, and the keys they leave unmasked or need
+    const int c0 = 16 * kPer * wave;
+    const bool live = c0 < t.nc;
+    const int rf = (t.gc0 + min(c0, t.nc - 1)) / p.G, rl = (t.gc0 + min(c0 + 16 * kPer, t.nc) - 1) / p.G;
+    const int pf = t.len - t.n + rf, pl = t.len - t.n + max(rl, rf);
+    const int all_lo = p.window_left < 0 ? 0 : max(pl - p.window_left, 0), all_hi = pf + 1;
+    const int any_lo = p.window_left < 0 ? 0 : max(pf - p.window_left, 0), any_hi = pl + 1;
+    // keys past which some row of the task is masked (for the staging's look at V)
+    const int task_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
+    const int task_hi = t.len - t.n + t.row0 + 1;
+
+    const char* const kb = p.k + t.hkv * p.k_hs + 16 * ld_ch;
+    const char* const vb = p.v + t.hkv * p.v_hs + 16 * ld_ch;
+    const int last_entry = p.table_cols - 1;
+    int en[kLd];
+    uint4 kq[kLd], vq[kLd];
+    uint32_t sc[kLd];
+    uint32_t ok = 0;  // bit i: key i of the thread's has a row
+    auto entries = [&](int base) {
+#pragma unroll
+      for (int i = 0; i < kLd; ++i) en[i] = t.table[min((base + ld_key + kStep * i) >> p.page_shift, last_entry)];
+    };
+    auto load = [&](int base) {
+      ok = 0;
+#pragma unroll
+      for (int i = 0; i < kLd; ++i) {
+        const int key = base + ld_key + kStep * i;
+        const bool in = key < t.khi && en[i] >= 0 && en[i] < p.num_pages;
+        ok |= in ? 1u << i : 0u;
+        const int64_t page = in ? en[i] : 0;
+        const int slot = in ? key & slot_mask : 0;
+        kq[i] = *reinterpret_cast<const uint4*>(kb + page * p.k_ps + slot * p.k_ss);
+        vq[i] = *reinterpret_cast<const uint4*>(vb + page * p.v_ps + slot * p.v_ss);
+        if (scaled) sc[i] = p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot];
+      }
+    };
+
+    Column st[kPer];
+    f32x4 acc[kPer][kDT];
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      st[c] = fresh_column();
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) acc[c][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int nblk = t.khi > t.klo ? ceil_div(t.khi - t.klo, kBlk) : 0;
+    if (nblk > 0) {
+      entries(t.klo);
+      load(t.klo);
+      entries(t.klo + kBlk);
+    }
+    __syncthreads();  // the run before is done with the tiles
+    for (int bi = 0; bi < nblk; ++bi) {
+      const int buf = bi & 1;
+      const int base = t.klo + bi * kBlk;
+      const bool part = base < task_lo || base + kBlk > task_hi;
+      {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kLd; ++i) {
+          const int key = ld_key + kStep * i;
+          const bool in = (ok >> i) & 1;
+          uint4* const kd = &s_k[buf][key * kKU];
+          uint4* const vd = &s_v[buf][key * kVU];
+          uint4 k2[2], v2[2];
+          if constexpr (kF8) {
+            const float ks = scaled ? __uint_as_float((sc[i] & 255u) << 23) : 1.0f;
+            const float vs = scaled ? __uint_as_float((sc[i] >> 8) << 23) : 1.0f;
+            decode16<kT>(kq[i], ks, k2[0], k2[1]);
+            decode16<kT>(vq[i], vs, v2[0], v2[1]);
+          } else {
+            k2[0] = kq[i];
+            v2[0] = vq[i];
+          }
+#pragma unroll
+          for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
+            if (!in) v2[h] = make_uint4(0, 0, 0, 0);
+            if (part) odd = odd || not_finite<kT>(v2[h]);
+            const int u = (kF8 ? 2 : 1) * ld_ch + h;
+            kd[u ^ (key & kSwz)] = k2[h];
+            vd[u] = v2[h];
+          }
+        }
+        uint64_t bad = 0;
+        if (!__all(ok == (1u << kLd) - 1u)) {
+#pragma unroll
+          for (int i = 0; i < kLd; ++i) {
+            const uint64_t no = __ballot(((ok >> i) & 1) == 0);
+#pragma unroll
+            for (int r = 0; r < 64 / kRowCh; ++r)
+              bad |= ((no >> (kRowCh * r)) & 1) << (kStep * i + (64 / kRowCh) * wave + r);
+          }
+        }
+        const uint32_t any_odd = part && __any(odd) ? 1 : 0;
+        if (lane == 0) {
+#pragma unroll
+          for (int h = 0; h < kSub; ++h) reinterpret_cast<uint32_t*>(&s_bad[buf][h])[wave] = static_cast<uint32_t>(bad >> (32 * h));
+          reinterpret_cast<uint32_t*>(&s_odd[buf])[wave] = any_odd;
+        }
+      }
+      __syncthreads();  // the block is visible; every wave is done with the block before last
+      if (bi + 1 < nblk) {
+        load(base + kBlk);
+        entries(base + 2 * kBlk);
+      }
+      if (live) {
+        const uint4 od = s_odd[buf];
+        const bool odd = (od.x | od.y | od.z | od.w) != 0;
+#pragma unroll
+        for (int sub = 0; sub < kSub; ++sub) {
+          const int kb0 = base + 32 * sub;
+          if (kb0 + 32 <= any_lo || kb0 >= min(any_hi, t.khi)) continue;
+          const uint4 bw = s_bad[buf][sub];
+          const uint32_t bad = __builtin_amdgcn_readfirstlane(bw.x | bw.y | bw.z | bw.w);
+          const bool masked = kb0 < all_lo || kb0 + 32 > all_hi || bad != 0;
+          const uint4* const kt = &s_k[buf][32 * sub * kKU];
+          const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][32 * sub * kVU]);
+          f32x4 s4[kPer][2];
+#pragma unroll
+          for (int c = 0; c < kPer; ++c)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) s4[c][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int s = 0; s < kS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint4 a = kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))];
+#pragma unroll
+              for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
+            }
+          float f[kPer][8];
+          uint32_t seen[kPer];
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) {
+            if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
+            seen[c] = 0xffffffffu;
+            if (masked) {
+              seen[c] = seen_keys(kb0, lc[c].lo, min(lc[c].hi, t.khi), bad, quad);
+              mask_scores(s4[c], seen[c]);
+            }
+            weigh(s4[c], scale, st[c], acc[c], f[c]);
+          }
+          if (masked && odd) {
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) pv_exact(acc[c], f[c], seen[c], vt, kVU * 8, quad, col);
+            continue;
+          }
+          uint4 pb[kPer];
+#pragma unroll
+          for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
+#pragma unroll
+          for (int dt = 0; dt < kDT; ++dt) {
+            const uint4 a = join(read_tr(vt + rd_v + 16 * dt), read_tr(vt + rd_v + 16 * kVU * 8 + 16 * dt));
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
+          }
+        }
+      }
+    }
+    if (!live) continue;
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      const float l = quad_sum(st[c].l);
+      if (!lc[c].ok) continue;
+      const float m = st[c].m * scale;
+      if (run.whole) {
+        const int64_t at = static_cast<int64_t>(t.q0 + lc[c].row) * p.Hq + t.hkv * p.G + lc[c].head;
+        const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+        uint16_t* o = p.out + at * D + 4 * quad;
+#pragma unroll
+        for (int dt = 0; dt < kDT; ++dt)
+          *reinterpret_cast<uint2*>(o + 16 * dt) = make_uint2(E::pack2(acc[c][dt][0] * inv, acc[c][dt][1] * inv),
+                                                              E::pack2(acc[c][dt][2] * inv, acc[c][dt][3] * inv));
+        if (quad == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+      } else {
+        const int64_t at = static_cast<int64_t>(run.slot) * (64 * kPer) + 16 * (kPer * wave + c) + col;
+        float* o = p.part_o + at * D + 4 * quad;
+#pragma unroll
+        for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[c][dt];
+        if (quad == 0) {
+          p.part_ml[at * 2] = m;
+          p.part_ml[at * 2 + 1] = l;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- combine ---
+
+// Stream form, second launch: the partial states of a task that several
+// workgroups shared.  One workgroup per (row, query head); the waves take every
+// fourth piece, four loads ahead.  Rows of whole tasks return at once.
+template <int D>
+__global__ void __launch_bounds__(256) combine_kernel(PagedParams p, int kc) {
+  constexpr int kV = D / 64;  // floats per lane
+  __shared__ int s_b;
+  __shared__ float s_o[4][D], s_m[4], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t row = blockIdx.x / p.Hq;
+  const int head = static_cast<int>(blockIdx.x - row * p.Hq);
+  if (tid == 0) s_b = -1;
+  __syncthreads();
+  for (int b = tid; b < p.B; b += 256)
+    if (p.qo_indptr[b] <= row && row < p.qo_indptr[b + 1]) s_b = b;
+  __syncthreads();
+  const int b = __builtin_amdgcn_readfirstlane(s_b);
+  if (b < 0) return;  // a row of no request
+  const PagedRequest r = paged_request(p, b);
+  if (r.n == 0) return;
+  const int total = p.plan[p.B], groups = stream_groups(p, total);
+  const int hkv = head / p.G;
+  const int gc = static_cast<int>(row - r.q0) * p.G + head - hkv * p.G;
+  const int ct = gc / p.cols, col = gc - ct * p.cols;
+  const int first = p.plan[b] + (hkv * r.tasks + ct) * r.units;
+  const int wa = stream_owner(first, total, groups), wb = stream_owner(first + r.units - 1, total, groups);
+  if (wa == wb) return;  // stored by its workgroup
+  const bool at_start = stream_begin(wa, total, groups) == first;
+  const int n = wb - wa + 1;
+  auto place = [&](int i) {
+    const int64_t slot = 2 * static_cast<int64_t>(wa + i) + (i == 0 && !at_start ? 1 : 0);
+    return slot * kc + col;
+  };
+  float m = -INFINITY, l = 0.0f, o[kV] = {};
+  constexpr int kB = 4;
+  for (int i0 = wave; i0 < n; i0 += 4 * kB) {
+    float pm[kB], pl[kB], po[kB][kV];
+#pragma unroll
+    for (int u = 0; u < kB; ++u) {
+      const int64_t at = place(min(i0 + 4 * u, n - 1));
+      pm[u] = p.part_ml[2 * at];
+      pl[u] = p.part_ml[2 * at + 1];
+#pragma unroll
+      for (int j = 0; j < kV; ++j) po[u][j] = p.part_o[at * D + 64 * j + lane];
+    }
+#pragma unroll
+    for (int u = 0; u < kB; ++u) {
+      if (i0 + 4 * u >= n) break;
+      const float mn = max3_nonan(m, pm[u], pm[u]);
+      const float fa = m == mn ? 1.0f : fast_exp2(m - mn), fb = pm[u] == mn ? 1.0f : fast_exp2(pm[u] - mn);
+      m = mn;
+      l = l * fa + pl[u] * fb;
+#pragma unroll
+      for (int j = 0; j < kV; ++j) o[j] = o[j] * fa + po[u][j] * fb;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kV; ++j) s_o[wave][64 * j + lane] = o[j];
+  if (lane == 0) {
+    s_m[wave] = m;
+    s_l[wave] = l;
+  }
+  __syncthreads();
+  float mx = s_m[0], lt = 0.0f;
+#pragma unroll
+  for (int w = 1; w < 4; ++w) mx = max3_nonan(mx, s_m[w], s_m[w]);
+  float f[4];
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    f[w] = s_m[w] == mx ? 1.0f : fast_exp2(s_m[w] - mx);
+    lt += s_l[w] * f[w];
+  }
+  const int64_t at = row * p.Hq + head;
+  const float inv = lt == 0.0f ? 0.0f : p.v_scale / lt;
+  for (int d = 2 * tid; d < D; d += 512) {
+    float y[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      y[0] += s_o[w][d] * f[w];
+      y[1] += s_o[w][d + 1] * f[w];
+    }
+    *reinterpret_cast<uint32_t*>(p.out + at * D + d) = E::pack2(y[0] * inv, y[1] * inv);
+  }
+  if (tid == 0) p.lse[at] = lt == 0.0f ? -INFINITY : (mx + fast_log2(lt)) * kLn2;
+}
+
+// ----------------------------------------------------------------- launch ---
+
+typedef void (*Kernel)(PagedParams);
+
+template <int D>
+Kernel body_kernel(int body) {
+  constexpr int kBlk = D > 128 ? 32 : 64;
+  switch (body) {
+    case kBodyStream16: return stream_kernel<D, 1>;
+    case kBodyStream32: return stream_kernel<D, 2>;
+    case kBodyTile64: return tile_kernel<D, 1, kBlk, 2>;
+    default: return tile_kernel<D, 2, kBlk, (D > 128 ? 1 : 2)>;
+  }
+}
+Kernel body_of(int D, int body) {
+  return D == 64 ? body_kernel<64>(body) : (D == 128 ? body_kernel<128>(body) : body_kernel<256>(body));
+}
+size_t plan_bytes(int B) { return sizeof(int) * (static_cast<size_t>(B) + 1); }
+
+}  // namespace
+
+#define MAC_PAGED_CAT2(a, b) a##b
+#define MAC_PAGED_CAT(a, b) MAC_PAGED_CAT2(a, b)
+
+namespace mac {
+
+int MAC_PAGED_CAT(paged_resident_, MAC_PAGED_NAME)(int D, int body, int B) {
+  int dev = 0, cus = 256, v = 0, per = 1;
+  if (hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0)
+    cus = v;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, reinterpret_cast<const void*>(body_of(D, body)), 256, plan_bytes(B)) != hipSuccess ||
+      per < 1)
+    per = 1;
+  return cus * per;
+}
+
+hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, int D, int body, int grid, hipStream_t stream) {
+  hipLaunchKernelGGL(body_of(D, body), dim3(grid), dim3(256), plan_bytes(p.B), stream, p);
+  if (p.stream) {
+    const dim3 rows(static_cast<unsigned>(p.total_q * p.Hq));
+    const int kc = kBodyCols[body];
+    if (D == 64) hipLaunchKernelGGL((combine_kernel<64>), rows, dim3(256), 0, stream, p, kc);
+    else if (D == 128) hipLaunchKernelGGL((combine_kernel<128>), rows, dim3(256), 0, stream, p, kc);
+    else hipLaunchKernelGGL((combine_kernel<256>), rows, dim3(256), 0, stream, p, kc);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace mac

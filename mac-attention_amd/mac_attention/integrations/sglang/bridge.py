@@ -32,6 +32,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _u32 = ctypes.c_uint32
+_f32 = ctypes.c_float
 _f64 = ctypes.c_double
 
 
@@ -84,6 +85,11 @@ EXPORTED_SYMBOLS = (
     "mac_prefill_window_attention_workspace",
     "mac_prefill_rectify_update_cache_bf16",
     "mac_decode_rope_preserve_q_bf16",
+    "mac_paged_cache_write_fp8",
+    "mac_paged_rope_write_fp8",
+    "mac_paged_cache_read_fp8",
+    "mac_paged_chunk_attention",
+    "mac_paged_chunk_attention_workspace",
     "mac_last_error",
     "mac_abi_version",
 )
@@ -115,6 +121,49 @@ class MacRectifyArgs(ctypes.Structure):
         ("request_length_len", _i32), ("B", _i32), ("R", _i32), ("M", _i32), ("Hq", _i32),
         ("Hkv", _i32), ("D", _i32), ("semantic_pos_ahead", _i32), ("front_sink_tokens", _i32),
         ("sink_mode", _i32), ("sm_scale", _f64),
+    ]
+
+
+class MacPagedCache(ctypes.Structure):
+    """ctypes mirror of ``MacPagedCache``."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("abi_version", _u32),
+        ("k_cache", _p), ("v_cache", _p), ("kv_scales", _p),
+        ("num_pages", _i64),
+        ("k_page_stride", _i64), ("k_slot_stride", _i64), ("k_head_stride", _i64),
+        ("v_page_stride", _i64), ("v_slot_stride", _i64), ("v_head_stride", _i64),
+        ("page_size", _i32), ("Hkv", _i32), ("D", _i32), ("cache_dtype", _i32),
+        ("k_scale", _f32), ("v_scale", _f32),
+    ]
+
+
+class MacPagedRopeArgs(ctypes.Structure):
+    """ctypes mirror of ``MacPagedRopeArgs``."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("abi_version", _u32),
+        ("q", _p), ("k", _p), ("v", _p),
+        ("q_stride0", _i64), ("q_stride1", _i64), ("k_stride0", _i64), ("k_stride1", _i64),
+        ("v_stride0", _i64), ("v_stride1", _i64),
+        ("q_out", _p), ("cos_sin_cache", _p), ("cos_sin_rows", _i64), ("cos_sin_stride0", _i64),
+        ("positions", _p), ("cache_locs", _p), ("tokens", _i64),
+        ("Hq", _i32), ("rotary_dim", _i32), ("is_neox", _i32), ("dtype", _i32),
+        ("positions_is_i64", _i32), ("cache_locs_is_i64", _i32),
+    ]
+
+
+class MacPagedAttentionArgs(ctypes.Structure):
+    """ctypes mirror of ``MacPagedAttentionArgs``."""
+
+    _fields_ = [
+        ("struct_size", _u32), ("abi_version", _u32),
+        ("q", _p), ("q_stride0", _i64), ("q_stride1", _i64),
+        ("qo_indptr", _p), ("kv_lens", _p), ("page_table", _p), ("table_stride", _i64), ("req_ids", _p),
+        ("out", _p), ("out_lse", _p),
+        ("total_q", _i64), ("B", _i32), ("Hq", _i32), ("table_rows", _i32), ("table_cols", _i32),
+        ("q_dtype", _i32), ("window_left", _i32),
+        ("sm_scale", _f64), ("logit_cap", _f64),
     ]
 
 
@@ -156,6 +205,17 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i32, _p, _i32, _p, _i32,
         _i64, _i32, _i32, _i32, _i32, _p]
     lib.mac_decode_rope_preserve_q_bf16.restype = ctypes.c_int
+    cache = ctypes.POINTER(MacPagedCache)
+    lib.mac_paged_cache_write_fp8.argtypes = [cache, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i32, _i64, _p]
+    lib.mac_paged_cache_write_fp8.restype = ctypes.c_int
+    lib.mac_paged_rope_write_fp8.argtypes = [cache, ctypes.POINTER(MacPagedRopeArgs), _p]
+    lib.mac_paged_rope_write_fp8.restype = ctypes.c_int
+    lib.mac_paged_cache_read_fp8.argtypes = [cache, _p, _i32, _i64, _p, _p, _i32, _p]
+    lib.mac_paged_cache_read_fp8.restype = ctypes.c_int
+    lib.mac_paged_chunk_attention_workspace.argtypes = [cache, ctypes.POINTER(MacPagedAttentionArgs)]
+    lib.mac_paged_chunk_attention_workspace.restype = ctypes.c_int64
+    lib.mac_paged_chunk_attention.argtypes = [cache, ctypes.POINTER(MacPagedAttentionArgs), _p, _i64, _p]
+    lib.mac_paged_chunk_attention.restype = ctypes.c_int
     if lib.mac_abi_version() != ABI_VERSION:
         raise RuntimeError(
             f"{path} has ABI version {lib.mac_abi_version()}, binding expects {ABI_VERSION}"
@@ -947,3 +1007,223 @@ class DecodeRopePreserveExtension:
 def load_mac_decode_rope_preserve_extension(verbose: bool = False) -> Any:
     """Reference bridge.py:273-290."""
     return DecodeRopePreserveExtension(load_library())
+
+
+# ------------------------------------------------------- paged 8-bit cache ---
+
+_DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_CACHE_SIZE = ctypes.sizeof(MacPagedCache)
+_PAGED_ROPE_SIZE = ctypes.sizeof(MacPagedRopeArgs)
+_PAGED_ATTENTION_SIZE = ctypes.sizeof(MacPagedAttentionArgs)
+_SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
+
+
+def _check_vector(t: torch.Tensor, name: str, device: torch.device, dtypes: tuple, n: int | None = None) -> None:
+    """A contiguous index vector on ``device`` (of n entries)."""
+    if (t.is_cuda and t.dtype in dtypes and t.dim() == 1 and t.is_contiguous() and t.device == device
+            and (n is None or t.shape[0] == n)):
+        return
+    _check(t.is_cuda, f"{name} must be CUDA")
+    _check(t.device == device, f"{name}: tensors must be on the same device")
+    _check(t.dtype in dtypes, f"{name} has wrong dtype")
+    _check(t.dim() == 1, f"{name} has wrong rank")
+    _check(t.is_contiguous(), f"{name} must be contiguous")
+    _check(n is None or t.shape[0] == n, f"{name} has wrong length")
+
+
+def _check_rows(t: torch.Tensor, name: str, device: torch.device, heads: int | None, d: int) -> None:
+    """Rows [tokens, heads, D], the last dimension contiguous."""
+    _check(t.is_cuda, f"{name} must be CUDA")
+    _check(t.device == device, f"{name}: tensors must be on the same device")
+    _check(t.dtype in (torch.bfloat16, torch.float16), f"{name} must be bfloat16 or float16")
+    _check(t.dim() == 3 and t.shape[2] == d and (heads is None or t.shape[1] == heads), f"{name} has wrong shape")
+    _check(t.stride(2) == 1, f"{name} must have contiguous last dimension")
+
+
+class PagedCacheExtension:
+    """Object returned by :func:`load_mac_paged_cache_extension`: an 8-bit paged
+    K/V cache (rows quantised as they are written, decode RoPE with the write,
+    rows read back) and attention of a chunk of new tokens over a paged cache of
+    8- or 16-bit rows.  No reference counterpart (its pool is bf16; FP8 K/V,
+    logit caps, other head sizes and larger groups are left to the engine).
+
+    Caches: k_cache, v_cache [pages, page_size, Hkv, D], float8_e4m3fn (attention:
+    or q's dtype), any page, slot and head strides of whole 16 bytes, page_size
+    a power of two (a pool [tokens, Hkv, D] is ``pool.unsqueeze(1)``).
+    kv_scales: uint8 or float8_e8m0fnu [pages, Hkv, page_size, 2], a row's K and
+    V scale as E8M0 bytes (2^(byte - 127)), or None: values are codes times the
+    static k_scale / v_scale."""
+
+    def __init__(self, lib: ctypes.CDLL):
+        self._lib = lib
+
+    @staticmethod
+    def _cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only: bool = True) -> MacPagedCache:
+        dt = k_cache.dtype
+        _check(k_cache.is_cuda and v_cache.is_cuda, "k_cache and v_cache must be CUDA")
+        _check(dt == torch.float8_e4m3fn or (not fp8_only and dt in (torch.bfloat16, torch.float16)),
+               "k_cache must be float8_e4m3fn" + ("" if fp8_only else ", bfloat16 or float16"))
+        _check(v_cache.dtype == dt, "v_cache must have k_cache's dtype")
+        _check(k_cache.dim() == 4, "k_cache must be [pages,page_size,Hkv,D]")
+        pages, page, hkv, d = k_cache.shape
+        _check(v_cache.shape == k_cache.shape, "v_cache must match k_cache")
+        _check(v_cache.device == k_cache.device, "v_cache: tensors must be on the same device")
+        ks, vs = k_cache.stride(), v_cache.stride()
+        _check(ks[3] == 1 and vs[3] == 1, "k_cache and v_cache must have contiguous last dimension")
+        if kv_scales is not None:
+            _check(kv_scales.is_cuda and kv_scales.device == k_cache.device,
+                   "kv_scales: tensors must be on the same device")
+            _check(dt == torch.float8_e4m3fn, "kv_scales belong to a float8_e4m3fn cache")
+            _check(kv_scales.dtype in _SCALE_DTYPES, "kv_scales must be uint8 or float8_e8m0fnu")
+            _check(kv_scales.shape == (pages, hkv, page, 2) and kv_scales.is_contiguous(),
+                   "kv_scales must be a contiguous [pages,Hkv,page_size,2] tensor")
+        n = k_cache.element_size()
+        return MacPagedCache(_CACHE_SIZE, ABI_VERSION, k_cache.data_ptr(), v_cache.data_ptr(),
+                             None if kv_scales is None else kv_scales.data_ptr(), pages,
+                             ks[0] * n, ks[1] * n, ks[2] * n, vs[0] * n, vs[1] * n, vs[2] * n, page, hkv, d,
+                             _DTYPE_CODES[dt], float(k_scale), float(v_scale))
+
+    def mac_paged_cache_write_fp8(self, k, v, k_cache, v_cache, kv_scales, cache_locs, k_scale: float = 1.0,
+                                  v_scale: float = 1.0) -> None:
+        """Quantises rows k, v [tokens, Hkv, D] (bf16 or fp16, any token and head
+        strides) into the slots cache_locs (int32 or int64: page * page_size +
+        slot; locs outside the cache are skipped, negative ones pad; a slot may
+        be named once per call)."""
+        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        dev = k_cache.device
+        _check_rows(k, "k", dev, c.Hkv, c.D)
+        _check_rows(v, "v", dev, c.Hkv, c.D)
+        _check(v.dtype == k.dtype and v.shape == k.shape, "v must match k")
+        n = k.shape[0]
+        _check_vector(cache_locs, "cache_locs", dev, (torch.int32, torch.int64), n)
+        with _on_device(dev):
+            rc = self._lib.mac_paged_cache_write_fp8(
+                ctypes.byref(c), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+                _DTYPE_CODES[k.dtype], cache_locs.data_ptr(), cache_locs.dtype == torch.int64, n, _stream(dev))
+        _raise_on(self._lib, rc)
+
+    def mac_paged_rope_write_fp8(self, q, k, v, k_cache, v_cache, kv_scales, cos_sin_cache, positions, cache_locs,
+                                 is_neox: bool = True, k_scale: float = 1.0, v_scale: float = 1.0, q_out=None):
+        """Decode RoPE with the write: returns q_out = RoPE(q) (q stays the
+        pre-RoPE query) and writes RoPE(k) and v quantised to the slots
+        cache_locs.  q [tokens, Hq, D], k, v [tokens, Hkv, D]; cos_sin_cache
+        float32 [positions, rotary_dim]; positions int32 or int64 (clamped into
+        the table)."""
+        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        dev = k_cache.device
+        _check_rows(q, "q", dev, None, c.D)
+        _check_rows(k, "k", dev, c.Hkv, c.D)
+        _check_rows(v, "v", dev, c.Hkv, c.D)
+        _check(q.dtype == k.dtype and v.dtype == k.dtype, "q, k and v must have the same dtype")
+        n, hq = q.shape[0], q.shape[1]
+        _check(k.shape[0] == n and v.shape[0] == n, "q/k/v batch mismatch")
+        _check(cos_sin_cache.is_cuda and cos_sin_cache.device == dev,
+               "cos_sin_cache: tensors must be on the same device")
+        _check(cos_sin_cache.dtype == torch.float32, "cos_sin_cache has wrong dtype")
+        _check(cos_sin_cache.dim() == 2, "cos_sin_cache must have rank 2")
+        _check(cos_sin_cache.stride(1) == 1, "cos_sin_cache must have contiguous last dimension")
+        rot = cos_sin_cache.shape[1]
+        _check(0 < rot <= c.D and rot % 2 == 0, "invalid rotary_dim")
+        ints = (torch.int32, torch.int64)
+        _check_vector(positions, "positions", dev, ints, n)
+        _check_vector(cache_locs, "cache_locs", dev, ints, n)
+        if q_out is None:
+            q_out = torch.empty((n, hq, c.D), device=dev, dtype=q.dtype)
+        _check(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.device == dev and q_out.is_contiguous(),
+               "q_out must be a contiguous tensor shaped like q")
+        a = MacPagedRopeArgs(_PAGED_ROPE_SIZE, ABI_VERSION, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0),
+                             q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), q_out.data_ptr(),
+                             cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], cos_sin_cache.stride(0),
+                             positions.data_ptr(), cache_locs.data_ptr(), n, hq, rot, bool(is_neox),
+                             _DTYPE_CODES[q.dtype], positions.dtype == torch.int64, cache_locs.dtype == torch.int64)
+        with _on_device(dev):
+            rc = self._lib.mac_paged_rope_write_fp8(ctypes.byref(c), ctypes.byref(a), _stream(dev))
+        _raise_on(self._lib, rc)
+        return q_out
+
+    def mac_paged_cache_read_fp8(self, k_cache, v_cache, kv_scales, kv_indices, dtype: torch.dtype = torch.bfloat16,
+                                 k_scale: float = 1.0, v_scale: float = 1.0, out_k=None, out_v=None):
+        """K and V [rows, Hkv, D] of the slots kv_indices (int32 or int64) in
+        dtype (bf16, fp16 or fp32); slots outside the cache read as zeros."""
+        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        dev = k_cache.device
+        _check(dtype in (torch.float32, torch.bfloat16, torch.float16), "dtype must be float32, bfloat16 or float16")
+        _check_vector(kv_indices, "kv_indices", dev, (torch.int32, torch.int64))
+        shape = (kv_indices.shape[0], c.Hkv, c.D)
+        outs = []
+        for name, t in (("out_k", out_k), ("out_v", out_v)):
+            if t is None:
+                t = torch.empty(shape, device=dev, dtype=dtype)
+            _check(t.shape == shape and t.dtype == dtype and t.device == dev and t.is_contiguous(),
+                   f"{name} must be a contiguous [rows,Hkv,D] tensor of dtype")
+            outs.append(t)
+        with _on_device(dev):
+            rc = self._lib.mac_paged_cache_read_fp8(
+                ctypes.byref(c), kv_indices.data_ptr(), kv_indices.dtype == torch.int64, shape[0], outs[0].data_ptr(),
+                outs[1].data_ptr(), _DTYPE_CODES[dtype], _stream(dev))
+        _raise_on(self._lib, rc)
+        return outs[0], outs[1]
+
+    def mac_paged_chunk_attention(self, q, k_cache, v_cache, qo_indptr, kv_lens, page_table, sm_scale: float,
+                                  kv_scales=None, k_scale: float = 1.0, v_scale: float = 1.0, window_left: int = -1,
+                                  logit_cap: float = 0.0, req_ids=None, out=None, out_lse=None):
+        """Causal attention of each request's new tokens over its cached keys
+        (the new ones among them): rows [qo_indptr[b], qo_indptr[b+1]) of q
+        [total_q, Hq, D] (bf16 or fp16) over kv_lens[b] keys in the pages of
+        page_table (int32 [rows, pages], row req_ids[b] or b).  Returns out
+        (q's dtype) and the natural-log lse (float32 [total_q, Hq]); rows that
+        see no key get 0 and -inf, rows of no request are left as they are."""
+        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only=False)
+        dev = k_cache.device
+        _check_rows(q, "q", dev, None, c.D)
+        _check(k_cache.dtype == torch.float8_e4m3fn or k_cache.dtype == q.dtype,
+               "k_cache must be float8_e4m3fn or of q's dtype")
+        total_q, hq = q.shape[0], q.shape[1]
+        _check(hq % c.Hkv == 0 if c.Hkv else False, "Hq must be a multiple of Hkv")
+        i32 = (torch.int32,)
+        _check_vector(qo_indptr, "qo_indptr", dev, i32)
+        batch = qo_indptr.shape[0] - 1
+        _check(batch >= 0, "qo_indptr must be [B+1]")
+        _check_vector(kv_lens, "kv_lens", dev, i32, batch)
+        if req_ids is not None:
+            _check_vector(req_ids, "req_ids", dev, i32, batch)
+        _check(page_table.is_cuda and page_table.device == dev, "page_table: tensors must be on the same device")
+        _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 [rows,pages]")
+        rows, cols = page_table.shape
+        _check(cols <= 1 or page_table.stride(1) == 1, "page_table must have contiguous rows")
+        _check(req_ids is not None or rows >= batch, "page_table has fewer rows than the batch")
+        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
+            q = q.contiguous()  # rows that 16-byte loads cannot read
+            if q.data_ptr() % 16:
+                q = q.clone()
+        if out is None:
+            out = torch.empty((total_q, hq, c.D), device=dev, dtype=q.dtype)
+        if out_lse is None:
+            out_lse = torch.empty((total_q, hq), device=dev, dtype=torch.float32)
+        _check(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous(),
+               "out must be a contiguous tensor shaped like q")
+        _check(out_lse.shape == (total_q, hq) and out_lse.dtype == torch.float32 and out_lse.device == dev
+               and out_lse.is_contiguous(), "out_lse must be contiguous f32 [total_q,Hq]")
+        a = MacPagedAttentionArgs(_PAGED_ATTENTION_SIZE, ABI_VERSION, q.data_ptr(), q.stride(0), q.stride(1),
+                                  qo_indptr.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
+                                  page_table.stride(0), None if req_ids is None else req_ids.data_ptr(),
+                                  out.data_ptr(), out_lse.data_ptr(), total_q, batch, hq, rows, cols,
+                                  _DTYPE_CODES[q.dtype], int(window_left), float(sm_scale), float(logit_cap))
+        lib = self._lib
+        with _on_device(dev):
+            # the partial states of keys that several workgroups share, from
+            # PyTorch's allocator (its stream-ordered reuse and graph pools keep
+            # it safe across streams and captures)
+            n = lib.mac_paged_chunk_attention_workspace(ctypes.byref(c), ctypes.byref(a))
+            ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
+            rc = lib.mac_paged_chunk_attention(ctypes.byref(c), ctypes.byref(a), None if ws is None else ws.data_ptr(),
+                                               max(n, 0), _stream(dev))
+        _raise_on(lib, rc)
+        return out, out_lse
+
+
+@lru_cache(maxsize=1)
+def load_mac_paged_cache_extension(verbose: bool = False) -> Any:
+    """No reference counterpart (the reference leaves FP8 K/V caches and their
+    attention to the serving engine)."""
+    return PagedCacheExtension(load_library())
