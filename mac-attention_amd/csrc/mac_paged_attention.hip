@@ -25,9 +25,9 @@
 //
 // Masked keys: keys past a row's range, past the cache or without a page get
 // s = -inf, and V of keys that no row may see is zeroed when staged.  A key that
-// some rows see and others do not is left in place: where such a block holds V
-// that is not finite (0 x NaN), its P V is summed without the masked keys
-// (pv_exact).
+// some rows see and others do not would reach them all through 0 x NaN if its V
+// is not finite: such a key is masked for every row and added at the end of the
+// run, for the rows that see it (add_key).
 
 #include <hip/hip_runtime.h>
 
@@ -100,12 +100,14 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 
 // Logit cap: raw scores to capped ones in log2 units, cap log2(e) tanh(x) with
 // tanh(x) = 1 - 2 / (1 + e^2x) (off by 2^-23 of the cap: the scores are fp32).
+__device__ __forceinline__ float capped(float x, float cap_in, float cap_out) {
+  return cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(x * cap_in)));
+}
 __device__ __forceinline__ void cap_scores(f32x4 (&c)[2], float cap_in, float cap_out) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      c[t][r] = cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(c[t][r] * cap_in)));
+    for (int r = 0; r < 4; ++r) c[t][r] = capped(c[t][r], cap_in, cap_out);
 }
 
 // The keys of 32 from `base` that a row with the range [lo, hi) sees, less
@@ -120,34 +122,6 @@ __device__ __forceinline__ void mask_scores(f32x4 (&c)[2], uint32_t seen) {
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) c[t][r] = (seen >> (16 * t + r)) & 1 ? c[t][r] : -INFINITY;
-}
-
-// O^T += V^T P^T of 32 keys without the masked ones, on the vector units: v
-// points at the block's first row (row_units 16-byte units apart).
-template <int kDT>
-__device__ __forceinline__ void pv_exact(f32x4 (&acc)[kDT], const float (&f)[8], uint32_t seen, const uint16_t* v,
-                                                   int row_halves, int quad, int col) {
-  float g[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) g[e] = (seen >> (16 * (e >> 2) + (e & 3))) & 1 ? f[e] : -1.0f;
-#pragma unroll 1
-  for (int kq = 0; kq < 4; ++kq) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float w = __shfl(g[e], 16 * kq + col);
-      const uint16_t* row = v + (16 * (e >> 2) + 4 * kq + (e & 3)) * row_halves + 4 * quad;
-#pragma unroll
-      for (int dt = 0; dt < kDT; ++dt) {
-        const uint2 x = *reinterpret_cast<const uint2*>(row + 16 * dt);
-        if (w >= 0.0f || w != w) {
-          acc[dt][0] += w * E::low(x.x);
-          acc[dt][1] += w * E::high(x.x);
-          acc[dt][2] += w * E::low(x.y);
-          acc[dt][3] += w * E::high(x.y);
-        }
-      }
-    }
-  }
 }
 
 // The rows and columns of one run as a lane sees them.
@@ -166,6 +140,62 @@ __device__ __forceinline__ LaneColumn lane_column(const PagedParams& p, const Pa
   k.lo = p.window_left < 0 ? 0 : max(pos - p.window_left, 0);
   k.hi = pos + 1;
   return k;
+}
+
+// Eight consecutive elements of a cached row from dim d, in fp32.
+__device__ __forceinline__ void row8(const char* row, int d, float scale, float (&x)[8]) {
+  uint4 w;
+  if constexpr (kF8) {
+    const uint2 c = *reinterpret_cast<const uint2*>(row + d);
+    w = make_uint4(E::decode2<false>(c.x, scale), E::decode2<true>(c.x, scale), E::decode2<false>(c.y, scale), E::decode2<true>(c.y, scale));
+  } else {
+    w = *reinterpret_cast<const uint4*>(row + 2 * d);
+  }
+  x[0] = E::low(w.x); x[1] = E::high(w.x); x[2] = E::low(w.y); x[3] = E::high(w.y);
+  x[4] = E::low(w.z); x[5] = E::high(w.z); x[6] = E::low(w.w); x[7] = E::high(w.w);
+}
+
+// Adds one key to the states of the rows that see it, in fp32 on the vector
+// units.  kSplitQ: q's chunks in the order of the 8-bit stream body.
+template <int D, int kPer, bool kSplitQ>
+__device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t, int key, const uint4 (&q)[kPer][D / 32],
+                                        const LaneColumn (&lc)[kPer], Column (&st)[kPer], f32x4 (&acc)[kPer][D / 16], int quad) {
+  const int64_t page = t.table[key >> p.page_shift];
+  const int slot = key & ((1 << p.page_shift) - 1);
+  const char* kr = p.k + page * p.k_ps + slot * p.k_ss + t.hkv * p.k_hs;
+  const char* vr = p.v + page * p.v_ps + slot * p.v_ss + t.hkv * p.v_hs;
+  const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot] : 0x7f7fu;
+  const float ks = __uint_as_float((sc & 255u) << 23), vs = __uint_as_float((sc >> 8) << 23);
+  float s[kPer] = {};
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    float k[8];
+    row8(kr, kSplitQ ? 64 * (i >> 1) + 16 * quad + 8 * (i & 1) : 32 * i + 8 * quad, ks, k);
+#pragma unroll
+    for (int c = 0; c < kPer; ++c) {
+      const uint32_t w[4] = {q[c][i].x, q[c][i].y, q[c][i].z, q[c][i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[c] = fmaf(E::high(w[e]), k[2 * e + 1], fmaf(E::low(w[e]), k[2 * e], s[c]));
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) {
+    float x = quad_sum(s[c]);
+    if (p.cap_out != 0.0f) x = capped(x, p.cap_in, p.cap_out);
+    if (key < lc[c].lo || key >= lc[c].hi) continue;
+    const float m = max3_nonan(st[c].m, x, x);
+    const float alpha = st[c].m == m ? 1.0f : fast_exp2((st[c].m - m) * p.q_scale);
+    const float f = x == m ? (m == -INFINITY ? 0.0f : 1.0f) : fast_exp2((x - m) * p.q_scale);
+    st[c].m = m;
+    st[c].l = st[c].l * alpha + (quad == 0 ? f : 0.0f);  // (a lane holds its part of the sum)
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) {
+      float v[8];
+      row8(vr, 16 * dt + 8 * (quad >> 1), vs, v);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[c][dt][r] = acc[c][dt][r] * alpha + f * ((quad & 1) ? v[4 + r] : v[r]);
+    }
+  }
 }
 
 // One run's place in the stream or in the task list.
@@ -213,6 +243,8 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre,
 // quad + 4 c), V through a tile of LDS of its own, which transposes it.  Two
 // blocks' registers: one computes while the other is in flight, and the page
 // entries go out a block ahead of the rows that need them.
+constexpr int kOddBlocks = 8;  // a wave's blocks at the rows' edges: a task has at most 32 rows, so 63 keys at either end
+
 template <int D, int kPer>
 __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
   constexpr int kS = D / 32;                  // k-steps of a score
@@ -225,6 +257,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
   __shared__ int s_tmp[4];
   __shared__ uint4 s_v[4][32 * kVU];
   __shared__ float s_m[4][kC], s_l[4][kC];
+  __shared__ uint2 s_odd[4][kOddBlocks];  // per wave: first key and key bits of blocks with keys to add apart
   static_assert(16 * kOut * 4 <= 32 * kVU * 16, "a wave's state fits its V tile");
 
   const int tid = threadIdx.x;
@@ -306,9 +339,11 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
       for (int dt = 0; dt < kDT; ++dt) acc[c][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
+    int n_odd = 0;  // blocks in s_odd
     auto compute = [&](int base, const Block& blk) {
       const uint32_t bad = __builtin_amdgcn_readfirstlane(blk.bad);
-      const bool masked = base < all_lo || base + 32 > all_hi || bad != 0;
+      const bool part = base < all_lo || base + 32 > all_hi;  // some row of the task does not see some key
+      const bool masked = part || bad != 0;
       float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
       if (scaled) {
 #pragma unroll
@@ -318,11 +353,12 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
         }
       }
       // V to LDS
-      bool odd = false;
+      uint32_t odd = 0;  // keys with V that is not finite
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the block before is read)
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const bool ok = !((bad >> (16 * i + col)) & 1);
+        bool odd_row = false;
 #pragma unroll
         for (int c = 0; c < kCh; ++c) {
           uint4 w[2];
@@ -332,13 +368,24 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
           for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
             if (masked) {
               if (!ok) w[h] = make_uint4(0, 0, 0, 0);
-              odd = odd || not_finite<kT>(w[h]);
+              if (part && not_finite<kT>(w[h])) {
+                w[h] = make_uint4(0, 0, 0, 0);
+                odd_row = true;
+              }
             }
             vw[16 * i * kVU + (kF8 ? 8 : 4) * c + h] = w[h];
           }
         }
+        if (part) {
+          const uint64_t o = __ballot(odd_row);
+          odd |= static_cast<uint32_t>((o | (o >> 16) | (o >> 32) | (o >> 48)) & 0xffffu) << (16 * i);
+        }
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      if (odd != 0) {
+        if (lane == 0) s_odd[wave][n_odd] = make_uint2(base, odd);
+        ++n_odd;
+      }
       // scores
       f32x4 s4[kPer][2];
 #pragma unroll
@@ -361,22 +408,13 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
             for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a[i][h], q[c][(kF8 ? 2 : 1) * ch + h], s4[c][i]);
       }
       float f[kPer][8];
-      uint32_t seen[kPer];
 #pragma unroll
       for (int c = 0; c < kPer; ++c) {
         if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
-        seen[c] = 0xffffffffu;
         if (masked) {
-          seen[c] = seen_keys(base, lc[c].lo, min(lc[c].hi, t.khi), bad, quad);
-          mask_scores(s4[c], seen[c]);
+          mask_scores(s4[c], seen_keys(base, lc[c].lo, min(lc[c].hi, t.khi), bad | odd, quad));
         }
         weigh(s4[c], scale, st[c], acc[c], f[c]);
-      }
-      if (masked && __any(odd)) {
-#pragma unroll
-        for (int c = 0; c < kPer; ++c)
-          pv_exact(acc[c], f[c], seen[c], reinterpret_cast<const uint16_t*>(&s_v[wave][0]), kVU * 8, quad, col);
-        return;
       }
       uint4 pb[kPer];
 #pragma unroll
@@ -417,6 +455,13 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
         base += 128;
         if (base >= t.khi) break;
       }
+    }
+
+    for (int i = 0; i < n_odd; ++i) {
+      const uint2 o = s_odd[wave][i];
+      const int first = __builtin_amdgcn_readfirstlane(o.x);
+      for (uint32_t left = __builtin_amdgcn_readfirstlane(o.y); left != 0; left &= left - 1)
+        add_key<D, kPer, kF8>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
     }
 
     // the four waves' states joined
@@ -503,12 +548,16 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
   constexpr int kLd = kBlk / kStep;
   constexpr int kSub = kBlk / 32;
   static_assert(kLd >= 1, "a block is at least one pass");
+  // blocks in which some row of the task misses some key: at either end of its
+  // keys the rows' 64 kPer - 1 and one block's
+  constexpr int kOdd = 2 * ((64 * kPer + kBlk - 1) / kBlk + 2);
   extern __shared__ int s_pre[];
   __shared__ int s_tmp[4];
   __shared__ uint4 s_k[2][kBlk * kKU];
   __shared__ uint4 s_v[2][kBlk * kVU];
   __shared__ uint4 s_bad[2][kSub];  // per wave: its keys (of each 32) without a row
-  __shared__ uint4 s_odd[2];        // per wave: V that is not finite among its rows (looked for in masked blocks)
+  __shared__ uint4 s_odd[kOdd][kSub];  // and, of the blocks at the rows' edges, its keys to add apart
+  __shared__ int s_odd_at[kOdd];       // the blocks' first keys
 
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -597,13 +646,14 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
       load(t.klo);
       entries(t.klo + kBlk);
     }
+    int n_part = 0;
     __syncthreads();  // the run before is done with the tiles
     for (int bi = 0; bi < nblk; ++bi) {
       const int buf = bi & 1;
       const int base = t.klo + bi * kBlk;
       const bool part = base < task_lo || base + kBlk > task_hi;
       {
-        bool odd = false;
+        uint32_t odd_rows = 0;  // bit i: the thread's part of row i
 #pragma unroll
         for (int i = 0; i < kLd; ++i) {
           const int key = ld_key + kStep * i;
@@ -623,28 +673,38 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
 #pragma unroll
           for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
             if (!in) v2[h] = make_uint4(0, 0, 0, 0);
-            if (part) odd = odd || not_finite<kT>(v2[h]);
+            if (part && not_finite<kT>(v2[h])) {
+              v2[h] = make_uint4(0, 0, 0, 0);
+              odd_rows |= 1u << i;
+            }
             const int u = (kF8 ? 2 : 1) * ld_ch + h;
             kd[u ^ (key & kSwz)] = k2[h];
             vd[u] = v2[h];
           }
         }
-        uint64_t bad = 0;
-        if (!__all(ok == (1u << kLd) - 1u)) {
+        // the wave's keys: 64 / kRowCh of each pass
+        uint64_t bad = 0, odd = 0;
+        if (!__all(ok == (1u << kLd) - 1u) || (part && __any(odd_rows))) {
 #pragma unroll
           for (int i = 0; i < kLd; ++i) {
-            const uint64_t no = __ballot(((ok >> i) & 1) == 0);
+            const uint64_t no = __ballot(((ok >> i) & 1) == 0), od = __ballot((odd_rows >> i) & 1);
 #pragma unroll
-            for (int r = 0; r < 64 / kRowCh; ++r)
-              bad |= ((no >> (kRowCh * r)) & 1) << (kStep * i + (64 / kRowCh) * wave + r);
+            for (int r = 0; r < 64 / kRowCh; ++r) {
+              const int key = kStep * i + (64 / kRowCh) * wave + r;
+              bad |= ((no >> (kRowCh * r)) & 1) << key;
+              odd |= static_cast<uint64_t>(((od >> (kRowCh * r)) & ((1ull << kRowCh) - 1)) != 0) << key;
+            }
           }
         }
-        const uint32_t any_odd = part && __any(odd) ? 1 : 0;
         if (lane == 0) {
 #pragma unroll
-          for (int h = 0; h < kSub; ++h) reinterpret_cast<uint32_t*>(&s_bad[buf][h])[wave] = static_cast<uint32_t>(bad >> (32 * h));
-          reinterpret_cast<uint32_t*>(&s_odd[buf])[wave] = any_odd;
+          for (int h = 0; h < kSub; ++h) {
+            reinterpret_cast<uint32_t*>(&s_bad[buf][h])[wave] = static_cast<uint32_t>((bad | odd) >> (32 * h));
+            if (part) reinterpret_cast<uint32_t*>(&s_odd[n_part][h])[wave] = static_cast<uint32_t>(odd >> (32 * h));
+          }
+          if (part && wave == 0) s_odd_at[n_part] = base;
         }
+        if (part) ++n_part;
       }
       __syncthreads();  // the block is visible; every wave is done with the block before last
       if (bi + 1 < nblk) {
@@ -652,8 +712,6 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
         entries(base + 2 * kBlk);
       }
       if (live) {
-        const uint4 od = s_odd[buf];
-        const bool odd = (od.x | od.y | od.z | od.w) != 0;
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub) {
           const int kb0 = base + 32 * sub;
@@ -677,21 +735,13 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
               for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
             }
           float f[kPer][8];
-          uint32_t seen[kPer];
-#pragma unroll
+    #pragma unroll
           for (int c = 0; c < kPer; ++c) {
             if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
-            seen[c] = 0xffffffffu;
-            if (masked) {
-              seen[c] = seen_keys(kb0, lc[c].lo, min(lc[c].hi, t.khi), bad, quad);
-              mask_scores(s4[c], seen[c]);
+                if (masked) {
+              mask_scores(s4[c], seen_keys(kb0, lc[c].lo, min(lc[c].hi, t.khi), bad, quad));
             }
             weigh(s4[c], scale, st[c], acc[c], f[c]);
-          }
-          if (masked && odd) {
-#pragma unroll
-            for (int c = 0; c < kPer; ++c) pv_exact(acc[c], f[c], seen[c], vt, kVU * 8, quad, col);
-            continue;
           }
           uint4 pb[kPer];
 #pragma unroll
@@ -706,6 +756,14 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
       }
     }
     if (!live) continue;
+    for (int i = 0; i < n_part; ++i)
+#pragma unroll 1
+      for (int h = 0; h < kSub; ++h) {
+        const uint4 o = s_odd[i][h];
+        const int first = __builtin_amdgcn_readfirstlane(s_odd_at[i]) + 32 * h;
+        for (uint32_t left = __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w); left != 0; left &= left - 1)
+          add_key<D, kPer, false>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
+      }
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       const float l = quad_sum(st[c].l);
