@@ -52,6 +52,7 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int G = Hq / c.Hkv;
   const int64_t cols = (total_q + B - 1) / B * G;  // columns of a request of average length
   ch.body = cols <= 16 ? kBodyStream16 : (cols <= 32 ? kBodyStream32 : (cols <= 64 ? kBodyTile64 : kBodyTile128));
+  if (c.D > 128) ch.body = std::max<int>(ch.body, kBodyTile64);  // (two blocks of such rows and the states exceed a wave's registers)
   const int room = kBodyCols[ch.body];
   ch.cols = G <= room ? room / G * G : room;  // whole rows where a row's heads fit
   ch.task_rows = G <= room ? ch.cols / G : 2;
@@ -128,6 +129,8 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   REQUIRE(((c->k_page_stride | c->k_slot_stride | c->k_head_stride | c->v_page_stride | c->v_slot_stride |
             c->v_head_stride) & 15) == 0,
           "cache strides must be multiples of 16 bytes");
+  for (const int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride})
+    REQUIRE(s >= 0 && s <= UINT_MAX, "cache strides must be less than 2^32 bytes");
   REQUIRE(aligned16(a->out), "out must be 16-byte aligned");
   Choice ch;
   REQUIRE(choose(*c, a->q_dtype, a->Hq, a->total_q, a->B, static_cast<int64_t>(a->table_cols) * c->page_size, ch),
@@ -155,12 +158,12 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   }
   p.q_ts = a->q_stride0;
   p.q_hs = a->q_stride1;
-  p.k_ps = c->k_page_stride;
-  p.k_ss = c->k_slot_stride;
-  p.k_hs = c->k_head_stride;
-  p.v_ps = c->v_page_stride;
-  p.v_ss = c->v_slot_stride;
-  p.v_hs = c->v_head_stride;
+  p.k_ps = static_cast<uint32_t>(c->k_page_stride);
+  p.k_ss = static_cast<uint32_t>(c->k_slot_stride);
+  p.k_hs = static_cast<uint32_t>(c->k_head_stride);
+  p.v_ps = static_cast<uint32_t>(c->v_page_stride);
+  p.v_ss = static_cast<uint32_t>(c->v_slot_stride);
+  p.v_hs = static_cast<uint32_t>(c->v_head_stride);
   p.table_stride = a->table_stride;
   p.total_q = a->total_q;
   p.num_pages = c->num_pages;

@@ -29,7 +29,7 @@ struct PagedParams {
   float* part_ml;  // [2 grid][cols][2] their reference points (log2 units) and sums
   int32_t* plan;   // [B + 1] units before each request, for the combining launch
   int64_t q_ts, q_hs;                          // elements
-  int64_t k_ps, k_ss, k_hs, v_ps, v_ss, v_hs;  // bytes
+  uint32_t k_ps, k_ss, k_hs, v_ps, v_ss, v_hs;  // bytes
   int64_t table_stride;
   int64_t total_q;
   int64_t num_pages;
@@ -166,6 +166,11 @@ __device__ __forceinline__ PagedTask paged_task(const PagedParams& p, int b, con
   return t;
 }
 
+// Registers of raw bits: native vectors (HIP's uint4 is a struct, whose arrays
+// the compiler left in scratch memory).
+typedef uint32_t pa_u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t pa_u32x4 __attribute__((ext_vector_type(4)));
+
 // 16-bit element types.
 typedef __bf16 pa_bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 pa_bf16x8 __attribute__((ext_vector_type(8)));
@@ -178,7 +183,7 @@ struct PagedElem;
 
 template <>
 struct PagedElem<MAC_DTYPE_BF16> {
-  static __device__ __forceinline__ pa_f32x4 mfma(const uint4& a, const uint4& b, pa_f32x4 c) {
+  static __device__ __forceinline__ pa_f32x4 mfma(const pa_u32x4& a, const pa_u32x4& b, pa_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(pa_bf16x8, a), __builtin_bit_cast(pa_bf16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -199,7 +204,7 @@ struct PagedElem<MAC_DTYPE_BF16> {
 
 template <>
 struct PagedElem<MAC_DTYPE_F16> {
-  static __device__ __forceinline__ pa_f32x4 mfma(const uint4& a, const uint4& b, pa_f32x4 c) {
+  static __device__ __forceinline__ pa_f32x4 mfma(const pa_u32x4& a, const pa_u32x4& b, pa_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(pa_f16x8, a), __builtin_bit_cast(pa_f16x8, b), c, 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -219,15 +224,15 @@ struct PagedElem<MAC_DTYPE_F16> {
 
 // Sixteen codes as two vectors of eight 16-bit values.
 template <int kT>
-__device__ __forceinline__ void decode16(const uint4& w, float s, uint4& a, uint4& b) {
+__device__ __forceinline__ void decode16(const pa_u32x4& w, float s, pa_u32x4& a, pa_u32x4& b) {
   typedef PagedElem<kT> E;
-  a = make_uint4(E::template decode2<false>(w.x, s), E::template decode2<true>(w.x, s),
-                 E::template decode2<false>(w.y, s), E::template decode2<true>(w.y, s));
-  b = make_uint4(E::template decode2<false>(w.z, s), E::template decode2<true>(w.z, s),
-                 E::template decode2<false>(w.w, s), E::template decode2<true>(w.w, s));
+  a = pa_u32x4{E::template decode2<false>(w.x, s), E::template decode2<true>(w.x, s),
+                 E::template decode2<false>(w.y, s), E::template decode2<true>(w.y, s)};
+  b = pa_u32x4{E::template decode2<false>(w.z, s), E::template decode2<true>(w.z, s),
+                 E::template decode2<false>(w.w, s), E::template decode2<true>(w.w, s)};
 }
 template <int kT>
-__device__ __forceinline__ bool not_finite(const uint4& w) {
+__device__ __forceinline__ bool not_finite(const pa_u32x4& w) {
   typedef PagedElem<kT> E;
   return E::not_finite(w.x) || E::not_finite(w.y) || E::not_finite(w.z) || E::not_finite(w.w);
 }

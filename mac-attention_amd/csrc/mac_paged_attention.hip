@@ -45,10 +45,13 @@ constexpr bool kF8 = MAC_PAGED_F8;
 typedef PagedElem<kT> E;
 typedef pa_f32x4 f32x4;
 
+// An index times a byte stride: both fit 32 bits, their product need not.
+__device__ __forceinline__ uint64_t at64(uint32_t i, uint32_t stride) { return static_cast<uint64_t>(i) * stride; }
+
 // Four dims of V, one row each of four: the transposing LDS read (lds_read_tr16)
 // of 16-bit elements of either type.
-__device__ __forceinline__ uint2 read_tr(const uint16_t* at) { return __builtin_bit_cast(uint2, lds_read_tr16(at)); }
-__device__ __forceinline__ uint4 join(const uint2& a, const uint2& b) { return make_uint4(a.x, a.y, b.x, b.y); }
+__device__ __forceinline__ pa_u32x2 read_tr(const uint16_t* at) { return __builtin_bit_cast(pa_u32x2, lds_read_tr16(at)); }
+__device__ __forceinline__ pa_u32x4 join(const pa_u32x2& a, const pa_u32x2& b) { return pa_u32x4{a.x, a.y, b.x, b.y}; }
 
 // Softmax state of one column tile: raw-score reference point m (-inf: no key
 // seen), the scaled score past which it moves, the lane's part of the sum, and
@@ -94,8 +97,8 @@ __device__ __forceinline__ void weigh(const f32x4 (&c)[2], float scale, Column& 
   s.l += sum;
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(E::pack2(f[0], f[1]), E::pack2(f[2], f[3]), E::pack2(f[4], f[5]), E::pack2(f[6], f[7]));
+__device__ __forceinline__ pa_u32x4 pack8(const float (&f)[8]) {
+  return pa_u32x4{E::pack2(f[0], f[1]), E::pack2(f[2], f[3]), E::pack2(f[4], f[5]), E::pack2(f[6], f[7])};
 }
 
 // Logit cap: raw scores to capped ones in log2 units, cap log2(e) tanh(x) with
@@ -144,12 +147,12 @@ __device__ __forceinline__ LaneColumn lane_column(const PagedParams& p, const Pa
 
 // Eight consecutive elements of a cached row from dim d, in fp32.
 __device__ __forceinline__ void row8(const char* row, int d, float scale, float (&x)[8]) {
-  uint4 w;
+  pa_u32x4 w;
   if constexpr (kF8) {
-    const uint2 c = *reinterpret_cast<const uint2*>(row + d);
-    w = make_uint4(E::decode2<false>(c.x, scale), E::decode2<true>(c.x, scale), E::decode2<false>(c.y, scale), E::decode2<true>(c.y, scale));
+    const pa_u32x2 c = *reinterpret_cast<const pa_u32x2*>(row + d);
+    w = pa_u32x4{E::decode2<false>(c.x, scale), E::decode2<true>(c.x, scale), E::decode2<false>(c.y, scale), E::decode2<true>(c.y, scale)};
   } else {
-    w = *reinterpret_cast<const uint4*>(row + 2 * d);
+    w = *reinterpret_cast<const pa_u32x4*>(row + 2 * d);
   }
   x[0] = E::low(w.x); x[1] = E::high(w.x); x[2] = E::low(w.y); x[3] = E::high(w.y);
   x[4] = E::low(w.z); x[5] = E::high(w.z); x[6] = E::low(w.w); x[7] = E::high(w.w);
@@ -158,13 +161,13 @@ __device__ __forceinline__ void row8(const char* row, int d, float scale, float 
 // Adds one key to the states of the rows that see it, in fp32 on the vector
 // units.  kSplitQ: q's chunks in the order of the 8-bit stream body.
 template <int D, int kPer, bool kSplitQ>
-__device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t, int key, const uint4 (&q)[kPer][D / 32],
+__device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t, int key, const pa_u32x4 (&q)[kPer][D / 32],
                                         const LaneColumn (&lc)[kPer], Column (&st)[kPer], f32x4 (&acc)[kPer][D / 16], int quad) {
-  const int64_t page = t.table[key >> p.page_shift];
+  const int page = t.table[key >> p.page_shift];
   const int slot = key & ((1 << p.page_shift) - 1);
-  const char* kr = p.k + page * p.k_ps + slot * p.k_ss + t.hkv * p.k_hs;
-  const char* vr = p.v + page * p.v_ps + slot * p.v_ss + t.hkv * p.v_hs;
-  const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot] : 0x7f7fu;
+  const char* kr = p.k + at64(page, p.k_ps) + at64(slot, p.k_ss) + at64(t.hkv, p.k_hs);
+  const char* vr = p.v + at64(page, p.v_ps) + at64(slot, p.v_ss) + at64(t.hkv, p.v_hs);
+  const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + slot] : 0x7f7fu;
   const float ks = __uint_as_float((sc & 255u) << 23), vs = __uint_as_float((sc >> 8) << 23);
   float s[kPer] = {};
 #pragma unroll
@@ -190,10 +193,16 @@ __device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t
     st[c].l = st[c].l * alpha + (quad == 0 ? f : 0.0f);  // (a lane holds its part of the sum)
 #pragma unroll
     for (int dt = 0; dt < D / 16; ++dt) {
-      float v[8];
-      row8(vr, 16 * dt + 8 * (quad >> 1), vs, v);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[c][dt][r] = acc[c][dt][r] * alpha + f * ((quad & 1) ? v[4 + r] : v[r]);
+      const int d = 16 * dt + 4 * quad;
+      pa_u32x2 w;
+      if constexpr (kF8) {
+        const uint32_t x = *reinterpret_cast<const uint32_t*>(vr + d);
+        w = pa_u32x2{E::decode2<false>(x, vs), E::decode2<true>(x, vs)};
+      } else {
+        w = *reinterpret_cast<const pa_u32x2*>(vr + 2 * d);
+      }
+      const f32x4 v = {E::low(w.x), E::high(w.x), E::low(w.y), E::high(w.y)};
+      acc[c][dt] = acc[c][dt] * alpha + v * f;
     }
   }
 }
@@ -238,26 +247,32 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre,
 
 // Few columns (16 kPer): the bytes of K and V bound the call, so the four waves
 // take different keys, 32 at a time, and meet once, at the end of a run.  A
-// wave needs no barrier on its way: K goes from memory straight into the
-// matrix operand's registers (lane (quad, col) loads key col, 16-byte chunks
-// quad + 4 c), V through a tile of LDS of its own, which transposes it.  Two
-// blocks' registers: one computes while the other is in flight, and the page
-// entries go out a block ahead of the rows that need them.
+// wave needs no barrier on its way: it loads whole rows (a quarter of a wave
+// reads one or two of them; operand order, a row per lane, takes eight times the
+// cache lookups per byte and ran at 4.2 TB/s where this runs at @@), and stages
+// them in tiles of LDS of its own, K as cached in XOR-swizzled chunks, V as 16-bit
+// values for the transposing reads.  Two blocks' registers: one computes while
+// the other is in flight, and the page entries go out a block ahead of the rows
+// that need them.
 constexpr int kOddBlocks = 8;  // a wave's blocks at the rows' edges: a task has at most 32 rows, so 63 keys at either end
 
 template <int D, int kPer>
 __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
-  constexpr int kS = D / 32;                  // k-steps of a score
-  constexpr int kCh = kF8 ? D / 64 : D / 32;  // 16-byte chunks of a row per lane
-  constexpr int kVU = D / 8 + 2;              // 16-byte units per staged V row
+  constexpr int kS = D / 32;                // k-steps of a score
+  constexpr int kRL = D * (kF8 ? 1 : 2) / 16;  // lanes (16-byte chunks) per cached row
+  constexpr int kRI = 64 / kRL;             // rows per load
+  constexpr int kNI = 32 / kRI;             // loads per block
+  constexpr int kW = kF8 ? 2 : 1;           // staged V vectors, and k-steps, per chunk
+  constexpr int kVU = D / 8 + 2;            // 16-byte units per staged V row
   constexpr int kDT = D / 16;
   constexpr int kC = 16 * kPer;
-  constexpr int kOut = D + 4;                 // floats per column of the joined state
+  constexpr int kOut = D + 4;               // floats per column of the joined state
   extern __shared__ int s_pre[];
   __shared__ int s_tmp[4];
-  __shared__ uint4 s_v[4][32 * kVU];
+  __shared__ pa_u32x4 s_k[4][32 * kRL];
+  __shared__ pa_u32x4 s_v[4][32 * kVU];
   __shared__ float s_m[4][kC], s_l[4][kC];
-  __shared__ uint2 s_odd[4][kOddBlocks];  // per wave: first key and key bits of blocks with keys to add apart
+  __shared__ pa_u32x2 s_odd[4][kOddBlocks];  // per wave: first key and key bits of blocks with keys to add apart
   static_assert(16 * kOut * 4 <= 32 * kVU * 16, "a wave's state fits its V tile");
 
   const int tid = threadIdx.x;
@@ -272,14 +287,19 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
   const int x0 = stream_begin(blockIdx.x, total, groups), x1 = stream_begin(blockIdx.x + 1, total, groups);
 
   const float scale = p.q_scale;
+  // (a static cache loads a word of K in the scale's place: a load that only
+  // some calls make would leave the waits behind it uncounted)
   const bool scaled = kF8 && p.scales != nullptr;
+  const uint16_t* const scales = scaled ? p.scales : reinterpret_cast<const uint16_t*>(p.k);
   const int slot_mask = (1 << p.page_shift) - 1;
-  uint4* const vw = &s_v[wave][0] + col * kVU + (kF8 ? 2 * quad : quad);
+  // chunk c of staged K row r lies at c ^ swizzle(r): eight rows' chunks on different banks
+  auto swizzle = [](int r) { return kRL >= 16 ? r & 15 : (kRL == 8 ? r & 7 : (r >> 2) & 3); };
+  const int ld_row = lane / kRL, ld_ch = lane % kRL;  // the lane's row of a load, its chunk
   const uint16_t* const vr = reinterpret_cast<const uint16_t*>(&s_v[wave][0]) + (4 * quad + (col >> 2)) * (kVU * 8) + 4 * (col & 3);
 
   struct Block {
-    uint4 k[2][kCh], v[2][kCh];
-    uint32_t sc[2];
+    pa_u32x4 k[kNI], v[kNI];
+    uint32_t sc;   // scale bytes of key lane % 32
     uint32_t bad;  // keys of the 32 without a row
   };
 
@@ -289,45 +309,38 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
     const PagedTask& t = run.task;
     // the wave's columns
     LaneColumn lc[kPer];
-    uint4 q[kPer][kS];
+    pa_u32x4 q[kPer][kS];
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       lc[c] = lane_column(p, t, 16 * c + col);
       const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
 #pragma unroll
       for (int s = 0; s < kS; ++s)
-        q[c][s] = *reinterpret_cast<const uint4*>(at + (kF8 ? 64 * (s >> 1) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad));
+        q[c][s] = *reinterpret_cast<const pa_u32x4*>(at + (kF8 ? 64 * (s >> 1) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad));
     }
     // keys that every row of the task sees
     const int all_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
     const int all_hi = t.len - t.n + t.row0 + 1;
 
-    const char* const kb = p.k + t.hkv * p.k_hs + 16 * quad;
-    const char* const vb = p.v + t.hkv * p.v_hs + 16 * quad;
+    const char* const kb = p.k + at64(t.hkv, p.k_hs) + 16 * ld_ch;
+    const char* const vb = p.v + at64(t.hkv, p.v_hs) + 16 * ld_ch;
     const int last_entry = p.table_cols - 1;
-    auto entries = [&](int base, int (&e)[2]) {
+    auto entry = [&](int base) { return t.table[min((base + (lane & 31)) >> p.page_shift, last_entry)]; };
+    auto load = [&](int base, int e, Block& blk) {
+      const int key = base + (lane & 31);
+      const bool ok = key < t.khi && e >= 0 && e < p.num_pages;
+      blk.bad = ~static_cast<uint32_t>(__ballot(ok));
+      const int page = ok ? e : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) e[i] = t.table[min((base + 16 * i + col) >> p.page_shift, last_entry)];
-    };
-    auto load = [&](int base, const int (&e)[2], Block& blk) {
-      uint32_t have = 0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = base + 16 * i + col;
-        const bool ok = key < t.khi && e[i] >= 0 && e[i] < p.num_pages;
-        have |= static_cast<uint32_t>(__ballot(ok) & 0xffffu) << (16 * i);
-        const int64_t page = ok ? e[i] : 0;
-        const int slot = ok ? key & slot_mask : 0;
-        const char* ka = kb + page * p.k_ps + slot * p.k_ss;
-        const char* va = vb + page * p.v_ps + slot * p.v_ss;
-#pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          blk.k[i][c] = *reinterpret_cast<const uint4*>(ka + 64 * c);
-          blk.v[i][c] = *reinterpret_cast<const uint4*>(va + 64 * c);
-        }
-        if (scaled) blk.sc[i] = p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot];
+      for (int i = 0; i < kNI; ++i) {
+        const int src = kRI * i + ld_row;
+        const uint32_t pg = __shfl(page, src);
+        const uint32_t slot = (base + src) & slot_mask;
+        blk.k[i] = *reinterpret_cast<const pa_u32x4*>(kb + at64(pg, p.k_ps) + at64(slot, p.k_ss));
+        blk.v[i] = *reinterpret_cast<const pa_u32x4*>(vb + at64(pg, p.v_ps) + at64(slot, p.v_ss));
       }
-      blk.bad = ~have;
+      if constexpr (kF8)
+        blk.sc = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + (key & slot_mask) : 0];
     };
 
     Column st[kPer];
@@ -344,46 +357,45 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
       const uint32_t bad = __builtin_amdgcn_readfirstlane(blk.bad);
       const bool part = base < all_lo || base + 32 > all_hi;  // some row of the task does not see some key
       const bool masked = part || bad != 0;
-      float ks[2] = {1.0f, 1.0f}, vs[2] = {1.0f, 1.0f};
-      if (scaled) {
+      const uint32_t sc = kF8 && scaled ? blk.sc : 0x7f7fu;
+      // rows to LDS
+      pa_u32x4 w[kNI][kW];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          ks[i] = __uint_as_float((blk.sc[i] & 255u) << 23);
-          vs[i] = __uint_as_float((blk.sc[i] >> 8) << 23);
-        }
+      for (int i = 0; i < kNI; ++i) {
+        if constexpr (kF8) decode16<kT>(blk.v[i], __uint_as_float((__shfl(sc, kRI * i + ld_row) >> 8) << 23), w[i][0], w[i][1]);
+        else w[i][0] = blk.v[i];
       }
-      // V to LDS
       uint32_t odd = 0;  // keys with V that is not finite
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the block before is read)
+      if (masked) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool ok = !((bad >> (16 * i + col)) & 1);
-        bool odd_row = false;
+        for (int i = 0; i < kNI; ++i) {
+          const bool ok = !((bad >> (kRI * i + ld_row)) & 1);
+          bool odd_row = false;
 #pragma unroll
-        for (int c = 0; c < kCh; ++c) {
-          uint4 w[2];
-          if constexpr (kF8) decode16<kT>(blk.v[i][c], vs[i], w[0], w[1]);
-          else w[0] = blk.v[i][c];
+          for (int h = 0; h < kW; ++h) {
+            const bool nf = ok && part && not_finite<kT>(w[i][h]);
+            odd_row = odd_row || nf;
+            const uint32_t z = ok && !nf ? 0xffffffffu : 0u;
+            w[i][h] = pa_u32x4{w[i][h].x & z, w[i][h].y & z, w[i][h].z & z, w[i][h].w & z};
+          }
+          const uint64_t o = __ballot(odd_row);
+          if (o != 0) {
 #pragma unroll
-          for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
-            if (masked) {
-              if (!ok) w[h] = make_uint4(0, 0, 0, 0);
-              if (part && not_finite<kT>(w[h])) {
-                w[h] = make_uint4(0, 0, 0, 0);
-                odd_row = true;
-              }
-            }
-            vw[16 * i * kVU + (kF8 ? 8 : 4) * c + h] = w[h];
+            for (int r = 0; r < kRI; ++r) odd |= static_cast<uint32_t>(((o >> (kRL * r)) & ((1ull << kRL) - 1)) != 0) << (kRI * i + r);
           }
         }
-        if (part) {
-          const uint64_t o = __ballot(odd_row);
-          odd |= static_cast<uint32_t>((o | (o >> 16) | (o >> 32) | (o >> 48)) & 0xffffu) << (16 * i);
-        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (the block before is read)
+#pragma unroll
+      for (int i = 0; i < kNI; ++i) {
+        const int r = kRI * i + ld_row;
+        s_k[wave][r * kRL + (ld_ch ^ swizzle(r))] = blk.k[i];
+#pragma unroll
+        for (int h = 0; h < kW; ++h) s_v[wave][r * kVU + kW * ld_ch + h] = w[i][h];
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       if (odd != 0) {
-        if (lane == 0) s_odd[wave][n_odd] = make_uint2(base, odd);
+        if (lane == 0) s_odd[wave][n_odd] = pa_u32x2{static_cast<uint32_t>(base), odd};
         ++n_odd;
       }
       // scores
@@ -392,20 +404,26 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
       for (int c = 0; c < kPer; ++c)
 #pragma unroll
         for (int i = 0; i < 2; ++i) s4[c][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      float ks[2] = {1.0f, 1.0f};
+      if constexpr (kF8) {
 #pragma unroll
-      for (int ch = 0; ch < kCh; ++ch) {
-        uint4 a[2][2];
+        for (int i = 0; i < 2; ++i) ks[i] = __uint_as_float((__shfl(sc, 16 * i + col) & 255u) << 23);
+      }
+#pragma unroll
+      for (int ch = 0; ch < kRL / 4; ++ch) {
+        pa_u32x4 a[2][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          if constexpr (kF8) decode16<kT>(blk.k[i][ch], ks[i], a[i][0], a[i][1]);
-          else a[i][0] = blk.k[i][ch];
+          const pa_u32x4 raw = s_k[wave][(16 * i + col) * kRL + ((4 * ch + quad) ^ swizzle(16 * i + col))];
+          if constexpr (kF8) decode16<kT>(raw, ks[i], a[i][0], a[i][1]);
+          else a[i][0] = raw;
         }
 #pragma unroll
-        for (int h = 0; h < (kF8 ? 2 : 1); ++h)
+        for (int h = 0; h < kW; ++h)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a[i][h], q[c][(kF8 ? 2 : 1) * ch + h], s4[c][i]);
+            for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a[i][h], q[c][kW * ch + h], s4[c][i]);
       }
       float f[kPer][8];
 #pragma unroll
@@ -416,12 +434,12 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
         }
         weigh(s4[c], scale, st[c], acc[c], f[c]);
       }
-      uint4 pb[kPer];
+      pa_u32x4 pb[kPer];
 #pragma unroll
       for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
 #pragma unroll
       for (int dt = 0; dt < kDT; ++dt) {
-        const uint4 a = join(read_tr(vr + 16 * dt), read_tr(vr + 16 * kVU * 8 + 16 * dt));
+        const pa_u32x4 a = join(read_tr(vr + 16 * dt), read_tr(vr + 16 * kVU * 8 + 16 * dt));
 #pragma unroll
         for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
       }
@@ -429,28 +447,24 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
 
     // the wave's blocks: every fourth of the run's
     Block ba, bb;
-    int ea[2], eb[2];
     int base = t.klo + 32 * wave;
     if (base < t.khi) {
-      entries(base, ea);
-      entries(base + 128, eb);
+      // (loads go out for a block past the run too, of the cache's first
+      // page: behind a branch the waits below could not count them)
+      int ea = entry(base), eb = entry(base + 128);
       load(base, ea, ba);
       while (true) {
-        if (base + 128 < t.khi) {
-          entries(base + 256, ea);
-          __builtin_amdgcn_sched_barrier(0);
-          load(base + 128, eb, bb);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        ea = entry(base + 256);
+        __builtin_amdgcn_sched_barrier(0);
+        load(base + 128, eb, bb);
+        __builtin_amdgcn_sched_barrier(0);
         compute(base, ba);
         base += 128;
         if (base >= t.khi) break;
-        if (base + 128 < t.khi) {
-          entries(base + 256, eb);
-          __builtin_amdgcn_sched_barrier(0);
-          load(base + 128, ea, ba);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+        eb = entry(base + 256);
+        __builtin_amdgcn_sched_barrier(0);
+        load(base + 128, ea, ba);
+        __builtin_amdgcn_sched_barrier(0);
         compute(base, bb);
         base += 128;
         if (base >= t.khi) break;
@@ -458,7 +472,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
     }
 
     for (int i = 0; i < n_odd; ++i) {
-      const uint2 o = s_odd[wave][i];
+      const pa_u32x2 o = s_odd[wave][i];
       const int first = __builtin_amdgcn_readfirstlane(o.x);
       for (uint32_t left = __builtin_amdgcn_readfirstlane(o.y); left != 0; left &= left - 1)
         add_key<D, kPer, kF8>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
@@ -510,8 +524,8 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
           const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
 #pragma unroll
           for (int i = 0; i < kDT; i += 4)
-            *reinterpret_cast<uint2*>(p.out + at * D + d0 + i) =
-                make_uint2(E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv));
+            *reinterpret_cast<pa_u32x2*>(p.out + at * D + d0 + i) =
+                pa_u32x2{E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv)};
           if (d0 == 0) p.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
         } else {
           const int64_t at = static_cast<int64_t>(run.slot) * kC + gcol;
@@ -553,10 +567,10 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
   constexpr int kOdd = 2 * ((64 * kPer + kBlk - 1) / kBlk + 2);
   extern __shared__ int s_pre[];
   __shared__ int s_tmp[4];
-  __shared__ uint4 s_k[2][kBlk * kKU];
-  __shared__ uint4 s_v[2][kBlk * kVU];
-  __shared__ uint4 s_bad[2][kSub];  // per wave: its keys (of each 32) without a row
-  __shared__ uint4 s_odd[kOdd][kSub];  // and, of the blocks at the rows' edges, its keys to add apart
+  __shared__ pa_u32x4 s_k[2][kBlk * kKU];
+  __shared__ pa_u32x4 s_v[2][kBlk * kVU];
+  __shared__ pa_u32x4 s_bad[2][kSub];  // per wave: its keys (of each 32) without a row
+  __shared__ pa_u32x4 s_odd[kOdd][kSub];  // and, of the blocks at the rows' edges, its keys to add apart
   __shared__ int s_odd_at[kOdd];       // the blocks' first keys
 
   const int tid = threadIdx.x;
@@ -574,7 +588,10 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
     x1 = stream_begin(blockIdx.x + 1, total, groups);
   }
   const float scale = p.q_scale;
+  // (a static cache loads a word of K in the scale's place: a load that only
+  // some calls make would leave the waits behind it uncounted)
   const bool scaled = kF8 && p.scales != nullptr;
+  const uint16_t* const scales = scaled ? p.scales : reinterpret_cast<const uint16_t*>(p.k);
   const int slot_mask = (1 << p.page_shift) - 1;
   // loader: thread t stages chunk t % kRowCh of keys t / kRowCh + kStep i
   const int ld_key = tid / kRowCh, ld_ch = tid % kRowCh;
@@ -586,13 +603,13 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
   while (next_run(p, s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
     LaneColumn lc[kPer];
-    uint4 q[kPer][kS];
+    pa_u32x4 q[kPer][kS];
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       lc[c] = lane_column(p, t, 16 * (kPer * wave + c) + col);
       const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
 #pragma unroll
-      for (int s = 0; s < kS; ++s) q[c][s] = *reinterpret_cast<const uint4*>(at + 32 * s + 8 * quad);
+      for (int s = 0; s < kS; ++s) q[c][s] = *reinterpret_cast<const pa_u32x4*>(at + 32 * s + 8 * quad);
     }
     // the wave's first and last row, and the keys they leave unmasked or need
     const int c0 = 16 * kPer * wave;
@@ -605,11 +622,11 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
     const int task_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
     const int task_hi = t.len - t.n + t.row0 + 1;
 
-    const char* const kb = p.k + t.hkv * p.k_hs + 16 * ld_ch;
-    const char* const vb = p.v + t.hkv * p.v_hs + 16 * ld_ch;
+    const char* const kb = p.k + at64(t.hkv, p.k_hs) + 16 * ld_ch;
+    const char* const vb = p.v + at64(t.hkv, p.v_hs) + 16 * ld_ch;
     const int last_entry = p.table_cols - 1;
     int en[kLd];
-    uint4 kq[kLd], vq[kLd];
+    pa_u32x4 kq[kLd], vq[kLd];
     uint32_t sc[kLd];
     uint32_t ok = 0;  // bit i: key i of the thread's has a row
     auto entries = [&](int base) {
@@ -623,11 +640,11 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
         const int key = base + ld_key + kStep * i;
         const bool in = key < t.khi && en[i] >= 0 && en[i] < p.num_pages;
         ok |= in ? 1u << i : 0u;
-        const int64_t page = in ? en[i] : 0;
+        const int page = in ? en[i] : 0;
         const int slot = in ? key & slot_mask : 0;
-        kq[i] = *reinterpret_cast<const uint4*>(kb + page * p.k_ps + slot * p.k_ss);
-        vq[i] = *reinterpret_cast<const uint4*>(vb + page * p.v_ps + slot * p.v_ss);
-        if (scaled) sc[i] = p.scales[((page * p.Hkv + t.hkv) << p.page_shift) + slot];
+        kq[i] = *reinterpret_cast<const pa_u32x4*>(kb + at64(page, p.k_ps) + at64(slot, p.k_ss));
+        vq[i] = *reinterpret_cast<const pa_u32x4*>(vb + at64(page, p.v_ps) + at64(slot, p.v_ss));
+        if constexpr (kF8) sc[i] = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + slot : 0];
       }
     };
 
@@ -658,9 +675,9 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
         for (int i = 0; i < kLd; ++i) {
           const int key = ld_key + kStep * i;
           const bool in = (ok >> i) & 1;
-          uint4* const kd = &s_k[buf][key * kKU];
-          uint4* const vd = &s_v[buf][key * kVU];
-          uint4 k2[2], v2[2];
+          pa_u32x4* const kd = &s_k[buf][key * kKU];
+          pa_u32x4* const vd = &s_v[buf][key * kVU];
+          pa_u32x4 k2[2], v2[2];
           if constexpr (kF8) {
             const float ks = scaled ? __uint_as_float((sc[i] & 255u) << 23) : 1.0f;
             const float vs = scaled ? __uint_as_float((sc[i] >> 8) << 23) : 1.0f;
@@ -672,9 +689,9 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
           }
 #pragma unroll
           for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
-            if (!in) v2[h] = make_uint4(0, 0, 0, 0);
+            if (!in) v2[h] = pa_u32x4{0, 0, 0, 0};
             if (part && not_finite<kT>(v2[h])) {
-              v2[h] = make_uint4(0, 0, 0, 0);
+              v2[h] = pa_u32x4{0, 0, 0, 0};
               odd_rows |= 1u << i;
             }
             const int u = (kF8 ? 2 : 1) * ld_ch + h;
@@ -716,10 +733,10 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
         for (int sub = 0; sub < kSub; ++sub) {
           const int kb0 = base + 32 * sub;
           if (kb0 + 32 <= any_lo || kb0 >= min(any_hi, t.khi)) continue;
-          const uint4 bw = s_bad[buf][sub];
+          const pa_u32x4 bw = s_bad[buf][sub];
           const uint32_t bad = __builtin_amdgcn_readfirstlane(bw.x | bw.y | bw.z | bw.w);
           const bool masked = kb0 < all_lo || kb0 + 32 > all_hi || bad != 0;
-          const uint4* const kt = &s_k[buf][32 * sub * kKU];
+          const pa_u32x4* const kt = &s_k[buf][32 * sub * kKU];
           const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][32 * sub * kVU]);
           f32x4 s4[kPer][2];
 #pragma unroll
@@ -730,7 +747,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
           for (int s = 0; s < kS; ++s)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const uint4 a = kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))];
+              const pa_u32x4 a = kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))];
 #pragma unroll
               for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
             }
@@ -743,12 +760,12 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
             }
             weigh(s4[c], scale, st[c], acc[c], f[c]);
           }
-          uint4 pb[kPer];
+          pa_u32x4 pb[kPer];
 #pragma unroll
           for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
 #pragma unroll
           for (int dt = 0; dt < kDT; ++dt) {
-            const uint4 a = join(read_tr(vt + rd_v + 16 * dt), read_tr(vt + rd_v + 16 * kVU * 8 + 16 * dt));
+            const pa_u32x4 a = join(read_tr(vt + rd_v + 16 * dt), read_tr(vt + rd_v + 16 * kVU * 8 + 16 * dt));
 #pragma unroll
             for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
           }
@@ -759,7 +776,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
     for (int i = 0; i < n_part; ++i)
 #pragma unroll 1
       for (int h = 0; h < kSub; ++h) {
-        const uint4 o = s_odd[i][h];
+        const pa_u32x4 o = s_odd[i][h];
         const int first = __builtin_amdgcn_readfirstlane(s_odd_at[i]) + 32 * h;
         for (uint32_t left = __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w); left != 0; left &= left - 1)
           add_key<D, kPer, false>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
@@ -775,8 +792,8 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
         uint16_t* o = p.out + at * D + 4 * quad;
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt)
-          *reinterpret_cast<uint2*>(o + 16 * dt) = make_uint2(E::pack2(acc[c][dt][0] * inv, acc[c][dt][1] * inv),
-                                                              E::pack2(acc[c][dt][2] * inv, acc[c][dt][3] * inv));
+          *reinterpret_cast<pa_u32x2*>(o + 16 * dt) = pa_u32x2{E::pack2(acc[c][dt][0] * inv, acc[c][dt][1] * inv),
+                                                              E::pack2(acc[c][dt][2] * inv, acc[c][dt][3] * inv)};
         if (quad == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + fast_log2(l)) * kLn2;
       } else {
         const int64_t at = static_cast<int64_t>(run.slot) * (64 * kPer) + 16 * (kPer * wave + c) + col;
@@ -889,8 +906,12 @@ template <int D>
 Kernel body_kernel(int body) {
   constexpr int kBlk = D > 128 ? 32 : 64;
   switch (body) {
-    case kBodyStream16: return stream_kernel<D, 1>;
-    case kBodyStream32: return stream_kernel<D, 2>;
+    case kBodyStream16:
+      if constexpr (D <= 128) return stream_kernel<D, 1>;
+      return nullptr;
+    case kBodyStream32:
+      if constexpr (D <= 128) return stream_kernel<D, 2>;
+      return nullptr;
     case kBodyTile64: return tile_kernel<D, 1, kBlk, 2>;
     default: return tile_kernel<D, 2, kBlk, (D > 128 ? 1 : 2)>;
   }
