@@ -251,9 +251,9 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre,
 // reads one or two of them; operand order, a row per lane, takes eight times the
 // cache lookups per byte and ran at 4.2 TB/s where this runs at @@), and stages
 // them in tiles of LDS of its own, K as cached in XOR-swizzled chunks, V as 16-bit
-// values for the transposing reads.  Two blocks' registers: one computes while
-// the other is in flight, and the page entries go out a block ahead of the rows
-// that need them.
+// values for the transposing reads.  A block's registers are free for the next
+// one's loads as soon as it is staged, so those are in flight while it is
+// computed; their page entries went out a block before.
 constexpr int kOddBlocks = 8;  // a wave's blocks at the rows' edges: a task has at most 32 rows, so 63 keys at either end
 
 template <int D, int kPer>
@@ -297,12 +297,6 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
   const int ld_row = lane / kRL, ld_ch = lane % kRL;  // the lane's row of a load, its chunk
   const uint16_t* const vr = reinterpret_cast<const uint16_t*>(&s_v[wave][0]) + (4 * quad + (col >> 2)) * (kVU * 8) + 4 * (col & 3);
 
-  struct Block {
-    pa_u32x4 k[kNI], v[kNI];
-    uint32_t sc;   // scale bytes of key lane % 32
-    uint32_t bad;  // keys of the 32 without a row
-  };
-
   int x = x0;
   Run run;
   while (next_run(p, s_pre, x0, x1, x, run)) {
@@ -325,22 +319,25 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
     const char* const kb = p.k + at64(t.hkv, p.k_hs) + 16 * ld_ch;
     const char* const vb = p.v + at64(t.hkv, p.v_hs) + 16 * ld_ch;
     const int last_entry = p.table_cols - 1;
+    // the block in flight: rows, scale bytes of key lane % 32, keys without a row
+    pa_u32x4 kq[kNI], vq[kNI];
+    uint32_t sc_next = 0x7f7fu, bad_next = 0;
     auto entry = [&](int base) { return t.table[min((base + (lane & 31)) >> p.page_shift, last_entry)]; };
-    auto load = [&](int base, int e, Block& blk) {
+    auto load = [&](int base, int e) {
       const int key = base + (lane & 31);
       const bool ok = key < t.khi && e >= 0 && e < p.num_pages;
-      blk.bad = ~static_cast<uint32_t>(__ballot(ok));
+      bad_next = ~static_cast<uint32_t>(__ballot(ok));
       const int page = ok ? e : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int src = kRI * i + ld_row;
         const uint32_t pg = __shfl(page, src);
         const uint32_t slot = (base + src) & slot_mask;
-        blk.k[i] = *reinterpret_cast<const pa_u32x4*>(kb + at64(pg, p.k_ps) + at64(slot, p.k_ss));
-        blk.v[i] = *reinterpret_cast<const pa_u32x4*>(vb + at64(pg, p.v_ps) + at64(slot, p.v_ss));
+        kq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(kb + at64(pg, p.k_ps) + at64(slot, p.k_ss)));
+        vq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(vb + at64(pg, p.v_ps) + at64(slot, p.v_ss)));
       }
       if constexpr (kF8)
-        blk.sc = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + (key & slot_mask) : 0];
+        sc_next = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + (key & slot_mask) : 0];
     };
 
     Column st[kPer];
@@ -353,17 +350,25 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
     }
 
     int n_odd = 0;  // blocks in s_odd
-    auto compute = [&](int base, const Block& blk) {
-      const uint32_t bad = __builtin_amdgcn_readfirstlane(blk.bad);
+    // the wave's blocks: every fourth of the run's
+    int base = t.klo + 32 * wave;
+    int e1 = 0;
+    if (base < t.khi) {
+      const int e0 = entry(base);
+      e1 = entry(base + 128);
+      load(base, e0);
+    }
+    for (; base < t.khi; base += 128) {
+      const uint32_t bad = __builtin_amdgcn_readfirstlane(bad_next);
       const bool part = base < all_lo || base + 32 > all_hi;  // some row of the task does not see some key
       const bool masked = part || bad != 0;
-      const uint32_t sc = kF8 && scaled ? blk.sc : 0x7f7fu;
+      const uint32_t sc = kF8 && scaled ? sc_next : 0x7f7fu;
       // rows to LDS
       pa_u32x4 w[kNI][kW];
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
-        if constexpr (kF8) decode16<kT>(blk.v[i], __uint_as_float((__shfl(sc, kRI * i + ld_row) >> 8) << 23), w[i][0], w[i][1]);
-        else w[i][0] = blk.v[i];
+        if constexpr (kF8) decode16<kT>(vq[i], __uint_as_float((__shfl(sc, kRI * i + ld_row) >> 8) << 23), w[i][0], w[i][1]);
+        else w[i][0] = vq[i];
       }
       uint32_t odd = 0;  // keys with V that is not finite
       if (masked) {
@@ -389,11 +394,17 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int r = kRI * i + ld_row;
-        s_k[wave][r * kRL + (ld_ch ^ swizzle(r))] = blk.k[i];
+        s_k[wave][r * kRL + (ld_ch ^ swizzle(r))] = kq[i];
 #pragma unroll
         for (int h = 0; h < kW; ++h) s_v[wave][r * kVU + kW * ld_ch + h] = w[i][h];
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_sched_barrier(0);
+      if (base + 128 < t.khi) {
+        load(base + 128, e1);
+        e1 = entry(base + 256);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       if (odd != 0) {
         if (lane == 0) s_odd[wave][n_odd] = pa_u32x2{static_cast<uint32_t>(base), odd};
         ++n_odd;
@@ -442,32 +453,6 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
         const pa_u32x4 a = join(read_tr(vr + 16 * dt), read_tr(vr + 16 * kVU * 8 + 16 * dt));
 #pragma unroll
         for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
-      }
-    };
-
-    // the wave's blocks: every fourth of the run's
-    Block ba, bb;
-    int base = t.klo + 32 * wave;
-    if (base < t.khi) {
-      // (loads go out for a block past the run too, of the cache's first
-      // page: behind a branch the waits below could not count them)
-      int ea = entry(base), eb = entry(base + 128);
-      load(base, ea, ba);
-      while (true) {
-        ea = entry(base + 256);
-        __builtin_amdgcn_sched_barrier(0);
-        load(base + 128, eb, bb);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(base, ba);
-        base += 128;
-        if (base >= t.khi) break;
-        eb = entry(base + 256);
-        __builtin_amdgcn_sched_barrier(0);
-        load(base + 128, ea, ba);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(base, bb);
-        base += 128;
-        if (base >= t.khi) break;
       }
     }
 
