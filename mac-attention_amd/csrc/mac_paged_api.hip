@@ -96,6 +96,7 @@ int check(const MacPagedCache* c, const MacPagedAttentionArgs* a) {
   REQUIRE(a->table_rows >= 0 && a->table_cols >= 0 &&
               static_cast<int64_t>(a->table_cols) * c->page_size < (int64_t{1} << 30),
           "page_table must name fewer than 2^30 keys per request");
+  REQUIRE(static_cast<int64_t>(c->Hkv) * c->page_size <= INT_MAX, "pages too large");
   REQUIRE(a->sm_scale > 0 && std::isfinite(a->sm_scale), "sm_scale must be positive");
   REQUIRE(a->logit_cap >= 0 && std::isfinite(a->logit_cap), "logit_cap must be >= 0");
   REQUIRE(c->k_scale > 0 && std::isfinite(c->k_scale) && c->v_scale > 0 && std::isfinite(c->v_scale),
@@ -126,10 +127,11 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   REQUIRE(a->page_table || a->table_cols == 0 || a->table_rows == 0, "null pointer argument");
   REQUIRE(aligned16(a->q) && ((a->q_stride0 | a->q_stride1) & 7) == 0, "q rows must be 16-byte aligned");
   REQUIRE(aligned16(c->k_cache) && aligned16(c->v_cache), "k_cache and v_cache must be 16-byte aligned");
-  REQUIRE(((c->k_page_stride | c->k_slot_stride | c->k_head_stride | c->v_page_stride | c->v_slot_stride |
-            c->v_head_stride) & 15) == 0,
+  REQUIRE(((c->k_page_stride | c->k_slot_stride | c->k_head_stride) & 15) == 0,
           "cache strides must be multiples of 16 bytes");
-  for (const int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride, c->v_page_stride, c->v_slot_stride, c->v_head_stride})
+  REQUIRE(c->k_page_stride == c->v_page_stride && c->k_slot_stride == c->v_slot_stride && c->k_head_stride == c->v_head_stride,
+          "k_cache and v_cache must have the same strides");
+  for (const int64_t s : {c->k_page_stride, c->k_slot_stride, c->k_head_stride})
     REQUIRE(s >= 0 && s <= UINT_MAX, "cache strides must be less than 2^32 bytes");
   REQUIRE(aligned16(a->out), "out must be 16-byte aligned");
   Choice ch;
@@ -158,15 +160,12 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   }
   p.q_ts = a->q_stride0;
   p.q_hs = a->q_stride1;
-  p.k_ps = static_cast<uint32_t>(c->k_page_stride);
-  p.k_ss = static_cast<uint32_t>(c->k_slot_stride);
-  p.k_hs = static_cast<uint32_t>(c->k_head_stride);
-  p.v_ps = static_cast<uint32_t>(c->v_page_stride);
-  p.v_ss = static_cast<uint32_t>(c->v_slot_stride);
-  p.v_hs = static_cast<uint32_t>(c->v_head_stride);
+  p.kv_ps = static_cast<uint32_t>(c->k_page_stride);
+  p.kv_ss = static_cast<uint32_t>(c->k_slot_stride);
+  p.kv_hs = static_cast<uint32_t>(c->k_head_stride);
   p.table_stride = a->table_stride;
   p.total_q = a->total_q;
-  p.num_pages = c->num_pages;
+  p.num_pages = static_cast<uint32_t>(c->num_pages);
   p.B = a->B;
   p.Hq = a->Hq;
   p.Hkv = c->Hkv;

@@ -29,10 +29,10 @@ struct PagedParams {
   float* part_ml;  // [2 grid][cols][2] their reference points (log2 units) and sums
   int32_t* plan;   // [B + 1] units before each request, for the combining launch
   int64_t q_ts, q_hs;                          // elements
-  uint32_t k_ps, k_ss, k_hs, v_ps, v_ss, v_hs;  // bytes
+  uint32_t kv_ps, kv_ss, kv_hs;  // bytes: page, slot and head strides of K and of V
   int64_t table_stride;
   int64_t total_q;
-  int64_t num_pages;
+  uint32_t num_pages;
   int B, Hq, Hkv, G;
   int table_rows, table_cols, page_shift;
   int window_left;  // < 0: none
@@ -47,6 +47,16 @@ struct PagedParams {
   float v_scale;
 };
 
+// The kernels read their parameters where the launch put them.  A fresh pointer
+// is opaque to the compiler: what is read through it is loaded where it is used,
+// not kept in scalar registers over the key loop (which spilled some 80 of them).
+typedef const __attribute__((address_space(4))) PagedParams PagedArgs;
+__device__ __forceinline__ PagedArgs& fresh_args() {
+  PagedArgs* a = (PagedArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *a;
+}
+
 // A request's rows, keys and tasks; all 0 for one whose rows do not lie in the
 // buffers.
 struct PagedRequest {
@@ -57,7 +67,7 @@ struct PagedRequest {
   int units;    // stream form: units per task
 };
 
-__device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int b) {
+__device__ __forceinline__ PagedRequest paged_request(PagedArgs& p, int b) {
   PagedRequest r;
   r.q0 = p.qo_indptr[b];
   const int q1 = p.qo_indptr[b + 1];
@@ -73,13 +83,13 @@ __device__ __forceinline__ PagedRequest paged_request(const PagedParams& p, int 
 }
 
 // Units (stream form) or tasks (plain form) of a request.
-__device__ __forceinline__ int paged_weight(const PagedParams& p, const PagedRequest& r) {
+__device__ __forceinline__ int paged_weight(PagedArgs& p, const PagedRequest& r) {
   return r.tasks * p.Hkv * (p.stream ? r.units : 1);
 }
 
 // Exclusive prefix of the requests' weights in s_pre[B + 1], by a workgroup of
 // 256 threads; ends with a barrier.  s_tmp: 4 entries.
-__device__ __forceinline__ void paged_plan(const PagedParams& p, int* s_pre, int* s_tmp) {
+__device__ __forceinline__ void paged_plan(PagedArgs& p, int* s_pre, int* s_tmp) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = ceil_div(p.B, 256);
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
@@ -124,7 +134,7 @@ __device__ __forceinline__ int paged_find(const int* s_pre, int B, int x) {
 }
 
 // Stream form: workgroups that get units, and the first unit of workgroup w.
-__device__ __forceinline__ int stream_groups(const PagedParams& p, int total) {
+__device__ __forceinline__ int stream_groups(PagedArgs& p, int total) {
   return min(p.grid, max(total / p.min_units, 1));
 }
 __device__ __forceinline__ int stream_begin(int w, int total, int groups) {
@@ -145,7 +155,7 @@ struct PagedTask {
   const int32_t* table;
 };
 
-__device__ __forceinline__ PagedTask paged_task(const PagedParams& p, int b, const PagedRequest& r, int index) {
+__device__ __forceinline__ PagedTask paged_task(PagedArgs& p, int b, const PagedRequest& r, int index) {
   PagedTask t;
   t.b = b;
   t.hkv = index / r.tasks;

@@ -54,47 +54,71 @@ __device__ __forceinline__ pa_u32x2 read_tr(const uint16_t* at) { return __built
 __device__ __forceinline__ pa_u32x4 join(const pa_u32x2& a, const pa_u32x2& b) { return pa_u32x4{a.x, a.y, b.x, b.y}; }
 
 // Softmax state of one column tile: raw-score reference point m (-inf: no key
-// seen), the scaled score past which it moves, the lane's part of the sum, and
-// whether a reference point of the wave is so large that m scale, rounded on its
-// own, would be off by whole powers of two (then (s - m) scale is formed instead
-// of one fma: 2^20 leaves 2^-4 of one).
+// seen), the scaled score past which it moves, the lane's part of the sum.
 struct Column {
   float m, past, l;
-  bool far;
 };
-__device__ __forceinline__ Column fresh_column() { return Column{-INFINITY, -INFINITY, 0.0f, false}; }
+__device__ __forceinline__ Column fresh_column() { return Column{-INFINITY, -INFINITY, 0.0f}; }
+// A reference point so large that m scale, rounded on its own, would be off by
+// whole powers of two (2^20 leaves 2^-4 of one): then (s - m) scale is formed
+// instead of one fma.
 constexpr float kFar = 1048576.0f;
 
-// Scores of 32 keys (c[t][r]: key 16 t + 4 quad + r) to weights in f[8], moving
-// the reference point where a score exceeds it by 2^8 (lazily: p <= 2^8 is as
-// exact, and most blocks rescale nothing).  Called by whole waves.
-template <int kDT>
-__device__ __forceinline__ void weigh(const f32x4 (&c)[2], float scale, Column& s, f32x4 (&acc)[kDT], float (&f)[8]) {
-  const float sv[8] = {c[0][0], c[0][1], c[0][2], c[0][3], c[1][0], c[1][1], c[1][2], c[1][3]};
-  const float top = max8_nonan(sv);
-  if (__any(top * scale > s.past)) {
-    const float bm = quad_max(top);
-    const float m_new = max3_nonan(s.m, bm, bm);
-    const float alpha = s.m == m_new ? 1.0f : fast_exp2((s.m - m_new) * scale);
-    s.m = m_new;
-    s.past = m_new * scale + 8.0f;
-    s.far = __any(fabsf(m_new) * scale > kFar && m_new != -INFINITY);
-    s.l *= alpha;
+// Scores of 32 keys (s[c][t][r]: key 16 t + 4 quad + r) to weights in f, moving
+// the reference points where a score exceeds one by 2^8 (lazily: p <= 2^8 is as
+// exact, and most blocks rescale nothing).  Called by whole waves; far: some
+// reference point of the wave is.  One branch each for all of the wave's columns:
+// the exponentials share a basic block with the products around them.
+template <int kPer, int kDT>
+__device__ __forceinline__ void weigh(const f32x4 (&s)[kPer][2], float scale, Column (&st)[kPer], bool& far,
+                                      f32x4 (&acc)[kPer][kDT], float (&f)[kPer][8]) {
+  float top[kPer];
+  bool past = false;
 #pragma unroll
-    for (int dt = 0; dt < kDT; ++dt) acc[dt] *= alpha;
+  for (int c = 0; c < kPer; ++c) {
+    const float sv[8] = {s[c][0][0], s[c][0][1], s[c][0][2], s[c][0][3], s[c][1][0], s[c][1][1], s[c][1][2], s[c][1][3]};
+    top[c] = max8_nonan(sv);
+    past = past || top[c] * scale > st[c].past;
   }
-  const float mo = s.m == -INFINITY ? 0.0f : -s.m * scale;
-  float sum = 0.0f;
-  if (s.far) {
+  if (__any(past)) {
+    bool big = false;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fast_exp2((s.m == -INFINITY ? sv[e] : sv[e] - s.m) * scale);
+    for (int c = 0; c < kPer; ++c) {
+      const float bm = quad_max(top[c]);
+      const float m_new = max3_nonan(st[c].m, bm, bm);
+      const float alpha = st[c].m == m_new ? 1.0f : fast_exp2((st[c].m - m_new) * scale);
+      st[c].m = m_new;
+      st[c].past = m_new * scale + 8.0f;
+      big = big || (fabsf(m_new) * scale > kFar && m_new != -INFINITY);
+      st[c].l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < kDT; ++dt) acc[c][dt] *= alpha;
+    }
+    far = __any(big);
+  }
+  if (far) {
+#pragma unroll
+    for (int c = 0; c < kPer; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[c][e] = (st[c].m == -INFINITY ? s[c][e >> 2][e & 3] : s[c][e >> 2][e & 3] - st[c].m) * scale;
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = fast_exp2(fmaf(sv[e], scale, mo));
+    for (int c = 0; c < kPer; ++c) {
+      const float mo = st[c].m == -INFINITY ? 0.0f : -st[c].m * scale;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[c][e] = fmaf(s[c][e >> 2][e & 3], scale, mo);
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sum += f[e];
-  s.l += sum;
+  for (int c = 0; c < kPer; ++c) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      f[c][e] = fast_exp2(f[c][e]);
+      sum = e == 0 ? f[c][e] : sum + f[c][e];
+    }
+    st[c].l += sum;
+  }
 }
 
 __device__ __forceinline__ pa_u32x4 pack8(const float (&f)[8]) {
@@ -127,23 +151,15 @@ __device__ __forceinline__ void mask_scores(f32x4 (&c)[2], uint32_t seen) {
     for (int r = 0; r < 4; ++r) c[t][r] = (seen >> (16 * t + r)) & 1 ? c[t][r] : -INFINITY;
 }
 
-// The rows and columns of one run as a lane sees them.
-struct LaneColumn {
-  int row, head;  // in the request, in the group
-  bool ok;
-  int lo, hi;  // keys the row sees
-};
-__device__ __forceinline__ LaneColumn lane_column(const PagedParams& p, const PagedTask& t, int c) {
-  LaneColumn k;
-  k.ok = c < t.nc;
-  const int gc = t.gc0 + min(c, t.nc - 1);  // (a column past the task computes its last one and stores nothing)
-  k.row = gc / p.G;
-  k.head = gc - k.row * p.G;
-  const int pos = t.len - t.n + k.row;
-  k.lo = p.window_left < 0 ? 0 : max(pos - p.window_left, 0);
-  k.hi = pos + 1;
-  return k;
+// Column c of a task: its row in the request and head in the group (a column past
+// the task computes its last one and stores nothing).
+__device__ __forceinline__ void lane_column(PagedArgs& p, const PagedTask& t, int c, int& row, int& head) {
+  const int gc = t.gc0 + min(c, t.nc - 1);
+  row = gc / p.G;
+  head = gc - row * p.G;
 }
+// First key that the row at a position sees.
+__device__ __forceinline__ int first_key(int pos, int window) { return window < 0 ? 0 : max(pos - window, 0); }
 
 // Eight consecutive elements of a cached row from dim d, in fp32.
 __device__ __forceinline__ void row8(const char* row, int d, float scale, float (&x)[8]) {
@@ -161,12 +177,13 @@ __device__ __forceinline__ void row8(const char* row, int d, float scale, float 
 // Adds one key to the states of the rows that see it, in fp32 on the vector
 // units.  kSplitQ: q's chunks in the order of the 8-bit stream body.
 template <int D, int kPer, bool kSplitQ>
-__device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t, int key, const pa_u32x4 (&q)[kPer][D / 32],
-                                        const LaneColumn (&lc)[kPer], Column (&st)[kPer], f32x4 (&acc)[kPer][D / 16], int quad) {
+__device__ __forceinline__ void add_key(PagedArgs& p, const PagedTask& t, int key, const pa_u32x4 (&q)[kPer][D / 32],
+                                        const int (&pos)[kPer], Column (&st)[kPer], f32x4 (&acc)[kPer][D / 16], int quad) {
   const int page = t.table[key >> p.page_shift];
   const int slot = key & ((1 << p.page_shift) - 1);
-  const char* kr = p.k + at64(page, p.k_ps) + at64(slot, p.k_ss) + at64(t.hkv, p.k_hs);
-  const char* vr = p.v + at64(page, p.v_ps) + at64(slot, p.v_ss) + at64(t.hkv, p.v_hs);
+  const uint64_t row = at64(page, p.kv_ps) + at64(slot, p.kv_ss) + at64(t.hkv, p.kv_hs);
+  const char* kr = p.k + row;
+  const char* vr = p.v + row;
   const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + slot] : 0x7f7fu;
   const float ks = __uint_as_float((sc & 255u) << 23), vs = __uint_as_float((sc >> 8) << 23);
   float s[kPer] = {};
@@ -185,7 +202,7 @@ __device__ __forceinline__ void add_key(const PagedParams& p, const PagedTask& t
   for (int c = 0; c < kPer; ++c) {
     float x = quad_sum(s[c]);
     if (p.cap_out != 0.0f) x = capped(x, p.cap_in, p.cap_out);
-    if (key < lc[c].lo || key >= lc[c].hi) continue;
+    if (key < first_key(pos[c], p.window_left) || key > pos[c]) continue;
     const float m = max3_nonan(st[c].m, x, x);
     const float alpha = st[c].m == m ? 1.0f : fast_exp2((st[c].m - m) * p.q_scale);
     const float f = x == m ? (m == -INFINITY ? 0.0f : 1.0f) : fast_exp2((x - m) * p.q_scale);
@@ -214,13 +231,19 @@ struct Run {
   int slot;    // else the partial state's place
 };
 
-// Run `i` of this workgroup.  Stream form: x is the unit it starts at (moved
+// This workgroup's next run.  Stream form: x is the unit it starts at (moved
 // past the run); plain form: the task number.  False: no more.
-__device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre, int x0, int x1, int& x, Run& r) {
+__device__ __forceinline__ bool next_run(PagedArgs& p, const int* s_pre, int x0, int x1, int& x, Run& r) {
   if (x >= x1) return false;
   const int b = __builtin_amdgcn_readfirstlane(paged_find(s_pre, p.B, x));
-  const PagedRequest q = paged_request(p, b);
-  const int at = x - s_pre[b];
+  PagedRequest q = paged_request(p, b);
+  q.q0 = __builtin_amdgcn_readfirstlane(q.q0);
+  q.n = __builtin_amdgcn_readfirstlane(q.n);
+  q.len = __builtin_amdgcn_readfirstlane(q.len);
+  q.keys = __builtin_amdgcn_readfirstlane(q.keys);
+  q.tasks = __builtin_amdgcn_readfirstlane(q.tasks);
+  q.units = __builtin_amdgcn_readfirstlane(q.units);
+  const int at = x - __builtin_amdgcn_readfirstlane(s_pre[b]);
   if (!p.stream) {
     // longest rows first within a request, its KV heads side by side
     const int index = at / p.Hkv, h = at - index * p.Hkv;
@@ -257,7 +280,7 @@ __device__ __forceinline__ bool next_run(const PagedParams& p, const int* s_pre,
 constexpr int kOddBlocks = 8;  // a wave's blocks at the rows' edges: a task has at most 32 rows, so 63 keys at either end
 
 template <int D, int kPer>
-__global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
+__global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   constexpr int kS = D / 32;                // k-steps of a score
   constexpr int kRL = D * (kF8 ? 1 : 2) / 16;  // lanes (16-byte chunks) per cached row
   constexpr int kRI = 64 / kRL;             // rows per load
@@ -278,20 +301,15 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
-  paged_plan(p, s_pre, s_tmp);
-  const int total = s_pre[p.B];
-  const int groups = stream_groups(p, total);
+  PagedArgs& a0 = fresh_args();
+  paged_plan(a0, s_pre, s_tmp);
+  const int total = __builtin_amdgcn_readfirstlane(s_pre[a0.B]);
+  const int groups = stream_groups(a0, total);
   if (blockIdx.x == 0)
-    for (int b = tid; b <= p.B; b += 256) p.plan[b] = s_pre[b];
+    for (int b = tid; b <= a0.B; b += 256) a0.plan[b] = s_pre[b];
   if (static_cast<int>(blockIdx.x) >= groups) return;
   const int x0 = stream_begin(blockIdx.x, total, groups), x1 = stream_begin(blockIdx.x + 1, total, groups);
 
-  const float scale = p.q_scale;
-  // (a static cache loads a word of K in the scale's place: a load that only
-  // some calls make would leave the waits behind it uncounted)
-  const bool scaled = kF8 && p.scales != nullptr;
-  const uint16_t* const scales = scaled ? p.scales : reinterpret_cast<const uint16_t*>(p.k);
-  const int slot_mask = (1 << p.page_shift) - 1;
   // chunk c of staged K row r lies at c ^ swizzle(r): eight rows' chunks on different banks
   auto swizzle = [](int r) { return kRL >= 16 ? r & 15 : (kRL == 8 ? r & 7 : (r >> 2) & 3); };
   const int ld_row = lane / kRL, ld_ch = lane % kRL;  // the lane's row of a load, its chunk
@@ -299,45 +317,57 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
 
   int x = x0;
   Run run;
-  while (next_run(p, s_pre, x0, x1, x, run)) {
+  while (next_run(fresh_args(), s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
+    PagedArgs& p = fresh_args();
+    const float scale = p.q_scale;
+    const int window = p.window_left;
+    // (a static cache loads a word of K in the scale's place: a load that only
+    // some calls make would leave the waits behind it uncounted)
+    const bool scaled = kF8 && p.scales != nullptr;
+    const uint16_t* const scales = scaled ? p.scales + (t.hkv << p.page_shift) : reinterpret_cast<const uint16_t*>(p.k);
+    const uint32_t sc_ps = scaled ? static_cast<uint32_t>(p.Hkv) << p.page_shift : 0;  // scale words per page
+    const int page_shift = p.page_shift, slot_mask = (1 << p.page_shift) - 1;
+    const uint32_t num_pages = p.num_pages, kv_ps = p.kv_ps, kv_ss = p.kv_ss;
     // the wave's columns
-    LaneColumn lc[kPer];
+    int pos[kPer];
     pa_u32x4 q[kPer][kS];
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
-      lc[c] = lane_column(p, t, 16 * c + col);
-      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
+      int row, head;
+      lane_column(p, t, 16 * c + col, row, head);
+      pos[c] = t.len - t.n + row;
+      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + row) * p.q_ts + (t.hkv * p.G + head) * p.q_hs;
 #pragma unroll
       for (int s = 0; s < kS; ++s)
         q[c][s] = *reinterpret_cast<const pa_u32x4*>(at + (kF8 ? 64 * (s >> 1) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad));
     }
     // keys that every row of the task sees
-    const int all_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
+    const int all_lo = first_key(t.len - t.n + t.row1, window);
     const int all_hi = t.len - t.n + t.row0 + 1;
 
-    const char* const kb = p.k + at64(t.hkv, p.k_hs) + 16 * ld_ch;
-    const char* const vb = p.v + at64(t.hkv, p.v_hs) + 16 * ld_ch;
+    const char* const kb = p.k + at64(t.hkv, p.kv_hs) + 16 * ld_ch;
+    const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
     // the block in flight: rows, scale bytes of key lane % 32, keys without a row
     pa_u32x4 kq[kNI], vq[kNI];
     uint32_t sc_next = 0x7f7fu, bad_next = 0;
-    auto entry = [&](int base) { return t.table[min((base + (lane & 31)) >> p.page_shift, last_entry)]; };
+    auto entry = [&](int base) {
+      return t.table[static_cast<uint32_t>(min((base + (lane & 31)) >> page_shift, last_entry))];
+    };
     auto load = [&](int base, int e) {
       const int key = base + (lane & 31);
-      const bool ok = key < t.khi && e >= 0 && e < p.num_pages;
+      const bool ok = key < t.khi && static_cast<uint32_t>(e) < num_pages;
       bad_next = ~static_cast<uint32_t>(__ballot(ok));
-      const int page = ok ? e : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
+      const uint32_t page = ok ? e : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int src = kRI * i + ld_row;
-        const uint32_t pg = __shfl(page, src);
-        const uint32_t slot = (base + src) & slot_mask;
-        kq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(kb + at64(pg, p.k_ps) + at64(slot, p.k_ss)));
-        vq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(vb + at64(pg, p.v_ps) + at64(slot, p.v_ss)));
+        const char* at = kb + at64(__shfl(page, src), kv_ps) + at64((base + src) & slot_mask, kv_ss);
+        kq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at));
+        vq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at + v_minus_k));
       }
-      if constexpr (kF8)
-        sc_next = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + (key & slot_mask) : 0];
+      if constexpr (kF8) sc_next = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
     };
 
     Column st[kPer];
@@ -349,6 +379,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
       for (int dt = 0; dt < kDT; ++dt) acc[c][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
+    bool far = false;
     int n_odd = 0;  // blocks in s_odd
     // the wave's blocks: every fourth of the run's
     int base = t.klo + 32 * wave;
@@ -436,15 +467,17 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
 #pragma unroll
             for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a[i][h], q[c][kW * ch + h], s4[c][i]);
       }
-      float f[kPer][8];
+      if (p.cap_out != 0.0f) {
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
-        if (masked) {
-          mask_scores(s4[c], seen_keys(base, lc[c].lo, min(lc[c].hi, t.khi), bad | odd, quad));
-        }
-        weigh(s4[c], scale, st[c], acc[c], f[c]);
+        for (int c = 0; c < kPer; ++c) cap_scores(s4[c], p.cap_in, p.cap_out);
       }
+      if (masked) {
+#pragma unroll
+        for (int c = 0; c < kPer; ++c)
+          mask_scores(s4[c], seen_keys(base, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad | odd, quad));
+      }
+      float f[kPer][8];
+      weigh(s4, scale, st, far, acc, f);
       pa_u32x4 pb[kPer];
 #pragma unroll
       for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
@@ -456,11 +489,12 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
       }
     }
 
+    PagedArgs& e = fresh_args();
     for (int i = 0; i < n_odd; ++i) {
       const pa_u32x2 o = s_odd[wave][i];
       const int first = __builtin_amdgcn_readfirstlane(o.x);
       for (uint32_t left = __builtin_amdgcn_readfirstlane(o.y); left != 0; left &= left - 1)
-        add_key<D, kPer, kF8>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
+        add_key<D, kPer, kF8>(e, t, first + __builtin_ctz(left), q, pos, st, acc, quad);
     }
 
     // the four waves' states joined
@@ -504,22 +538,23 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
           for (int j = 0; j < 4; ++j) r[i + j] = sum[j];
         }
         if (run.whole) {
-          const LaneColumn k = lane_column(p, t, gcol);
-          const int64_t at = static_cast<int64_t>(t.q0 + k.row) * p.Hq + t.hkv * p.G + k.head;
-          const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
+          int row, head;
+          lane_column(e, t, gcol, row, head);
+          const int64_t at = static_cast<int64_t>(t.q0 + row) * e.Hq + t.hkv * e.G + head;
+          const float inv = l == 0.0f ? 0.0f : e.v_scale / l;
 #pragma unroll
           for (int i = 0; i < kDT; i += 4)
-            *reinterpret_cast<pa_u32x2*>(p.out + at * D + d0 + i) =
+            *reinterpret_cast<pa_u32x2*>(e.out + at * D + d0 + i) =
                 pa_u32x2{E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv)};
-          if (d0 == 0) p.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
+          if (d0 == 0) e.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
         } else {
           const int64_t at = static_cast<int64_t>(run.slot) * kC + gcol;
 #pragma unroll
           for (int i = 0; i < kDT; i += 4)
-            *reinterpret_cast<f32x4*>(p.part_o + at * D + d0 + i) = f32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+            *reinterpret_cast<f32x4*>(e.part_o + at * D + d0 + i) = f32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
           if (d0 == 0) {
-            p.part_ml[at * 2] = mx;
-            p.part_ml[at * 2 + 1] = l;
+            e.part_ml[at * 2] = mx;
+            e.part_ml[at * 2 + 1] = l;
           }
         }
       }
@@ -536,7 +571,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams p) {
 // & 15) (& 7 for 64 dims) of its row, so that the 16 keys an operand reads lie
 // on different banks; V rows are padded by 32 bytes for the transposing reads.
 template <int D, int kPer, int kBlk, int kOcc>
-__global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
+__global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
   constexpr int kS = D / 32;
   constexpr int kDT = D / 16;
   constexpr int kKU = D / 8;               // 16-byte units per staged K row
@@ -546,6 +581,8 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
   constexpr int kStep = 256 / kRowCh;           // keys per pass of the workgroup
   constexpr int kLd = kBlk / kStep;
   constexpr int kSub = kBlk / 32;
+  constexpr int kW = kF8 ? 2 : 1;  // staged vectors per chunk
+  constexpr bool kAhead = D <= 128;  // (operands of 256 dims would take 128 registers)
   static_assert(kLd >= 1, "a block is at least one pass");
   // blocks in which some row of the task misses some key: at either end of its
   // keys the rows' 64 kPer - 1 and one block's
@@ -561,23 +598,18 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
-  paged_plan(p, s_pre, s_tmp);
-  const int total = s_pre[p.B];
+  PagedArgs& a0 = fresh_args();
+  paged_plan(a0, s_pre, s_tmp);
+  const int total = __builtin_amdgcn_readfirstlane(s_pre[a0.B]);
   int x0 = blockIdx.x, x1 = total;
-  if (p.stream) {
-    const int groups = stream_groups(p, total);
+  if (a0.stream) {
+    const int groups = stream_groups(a0, total);
     if (blockIdx.x == 0)
-      for (int b = tid; b <= p.B; b += 256) p.plan[b] = s_pre[b];
+      for (int b = tid; b <= a0.B; b += 256) a0.plan[b] = s_pre[b];
     if (static_cast<int>(blockIdx.x) >= groups) return;
     x0 = stream_begin(blockIdx.x, total, groups);
     x1 = stream_begin(blockIdx.x + 1, total, groups);
   }
-  const float scale = p.q_scale;
-  // (a static cache loads a word of K in the scale's place: a load that only
-  // some calls make would leave the waits behind it uncounted)
-  const bool scaled = kF8 && p.scales != nullptr;
-  const uint16_t* const scales = scaled ? p.scales : reinterpret_cast<const uint16_t*>(p.k);
-  const int slot_mask = (1 << p.page_shift) - 1;
   // loader: thread t stages chunk t % kRowCh of keys t / kRowCh + kStep i
   const int ld_key = tid / kRowCh, ld_ch = tid % kRowCh;
   // compute: the lane's V^T read position
@@ -585,30 +617,42 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
 
   int x = x0;
   Run run;
-  while (next_run(p, s_pre, x0, x1, x, run)) {
+  while (next_run(fresh_args(), s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
-    LaneColumn lc[kPer];
+    PagedArgs& p = fresh_args();
+    const float scale = p.q_scale;
+    const int window = p.window_left;
+    // (a static cache loads a word of K in the scale's place: a load that only
+    // some calls make would leave the waits behind it uncounted)
+    const bool scaled = kF8 && p.scales != nullptr;
+    const uint16_t* const scales = scaled ? p.scales + (t.hkv << p.page_shift) : reinterpret_cast<const uint16_t*>(p.k);
+    const uint32_t sc_ps = scaled ? static_cast<uint32_t>(p.Hkv) << p.page_shift : 0;  // scale words per page
+    const int page_shift = p.page_shift, slot_mask = (1 << p.page_shift) - 1;
+    const uint32_t num_pages = p.num_pages, kv_ps = p.kv_ps, kv_ss = p.kv_ss;
+    int pos[kPer];
     pa_u32x4 q[kPer][kS];
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
-      lc[c] = lane_column(p, t, 16 * (kPer * wave + c) + col);
-      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + lc[c].row) * p.q_ts + (t.hkv * p.G + lc[c].head) * p.q_hs;
+      int row, head;
+      lane_column(p, t, 16 * (kPer * wave + c) + col, row, head);
+      pos[c] = t.len - t.n + row;
+      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + row) * p.q_ts + (t.hkv * p.G + head) * p.q_hs;
 #pragma unroll
       for (int s = 0; s < kS; ++s) q[c][s] = *reinterpret_cast<const pa_u32x4*>(at + 32 * s + 8 * quad);
     }
     // the wave's first and last row, and the keys they leave unmasked or need
     const int c0 = 16 * kPer * wave;
     const bool live = c0 < t.nc;
-    const int rf = (t.gc0 + min(c0, t.nc - 1)) / p.G, rl = (t.gc0 + min(c0 + 16 * kPer, t.nc) - 1) / p.G;
-    const int pf = t.len - t.n + rf, pl = t.len - t.n + max(rl, rf);
-    const int all_lo = p.window_left < 0 ? 0 : max(pl - p.window_left, 0), all_hi = pf + 1;
-    const int any_lo = p.window_left < 0 ? 0 : max(pf - p.window_left, 0), any_hi = pl + 1;
+    const int pf = t.len - t.n + (t.gc0 + min(c0, t.nc - 1)) / p.G;
+    const int pl = t.len - t.n + (t.gc0 + min(c0 + 16 * kPer, t.nc) - 1) / p.G;  // (of no use to a wave that is not live)
+    const int all_lo = first_key(pl, window), all_hi = pf + 1;
+    const int any_lo = first_key(pf, window), any_hi = min(pl + 1, t.khi);
     // keys past which some row of the task is masked (for the staging's look at V)
-    const int task_lo = p.window_left < 0 ? 0 : max(t.len - t.n + t.row1 - p.window_left, 0);
+    const int task_lo = first_key(t.len - t.n + t.row1, window);
     const int task_hi = t.len - t.n + t.row0 + 1;
 
-    const char* const kb = p.k + at64(t.hkv, p.k_hs) + 16 * ld_ch;
-    const char* const vb = p.v + at64(t.hkv, p.v_hs) + 16 * ld_ch;
+    const char* const kb = p.k + at64(t.hkv, p.kv_hs) + 16 * ld_ch;
+    const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
     int en[kLd];
     pa_u32x4 kq[kLd], vq[kLd];
@@ -616,20 +660,21 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
     uint32_t ok = 0;  // bit i: key i of the thread's has a row
     auto entries = [&](int base) {
 #pragma unroll
-      for (int i = 0; i < kLd; ++i) en[i] = t.table[min((base + ld_key + kStep * i) >> p.page_shift, last_entry)];
+      for (int i = 0; i < kLd; ++i)
+        en[i] = t.table[static_cast<uint32_t>(min((base + ld_key + kStep * i) >> page_shift, last_entry))];
     };
     auto load = [&](int base) {
       ok = 0;
 #pragma unroll
       for (int i = 0; i < kLd; ++i) {
         const int key = base + ld_key + kStep * i;
-        const bool in = key < t.khi && en[i] >= 0 && en[i] < p.num_pages;
+        const bool in = key < t.khi && static_cast<uint32_t>(en[i]) < num_pages;
         ok |= in ? 1u << i : 0u;
-        const int page = in ? en[i] : 0;
-        const int slot = in ? key & slot_mask : 0;
-        kq[i] = *reinterpret_cast<const pa_u32x4*>(kb + at64(page, p.k_ps) + at64(slot, p.k_ss));
-        vq[i] = *reinterpret_cast<const pa_u32x4*>(vb + at64(page, p.v_ps) + at64(slot, p.v_ss));
-        if constexpr (kF8) sc[i] = scales[scaled ? ((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + slot : 0];
+        const uint32_t page = in ? en[i] : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
+        const char* at = kb + at64(page, kv_ps) + at64(key & slot_mask, kv_ss);
+        kq[i] = *reinterpret_cast<const pa_u32x4*>(at);
+        vq[i] = *reinterpret_cast<const pa_u32x4*>(at + v_minus_k);
+        if constexpr (kF8) sc[i] = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
       }
     };
 
@@ -649,6 +694,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
       entries(t.klo + kBlk);
     }
     int n_part = 0;
+    bool far = false;
     __syncthreads();  // the run before is done with the tiles
     for (int bi = 0; bi < nblk; ++bi) {
       const int buf = bi & 1;
@@ -656,37 +702,41 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
       const bool part = base < task_lo || base + kBlk > task_hi;
       {
         uint32_t odd_rows = 0;  // bit i: the thread's part of row i
+        const bool whole = __all(ok == (1u << kLd) - 1u);
 #pragma unroll
         for (int i = 0; i < kLd; ++i) {
           const int key = ld_key + kStep * i;
-          const bool in = (ok >> i) & 1;
           pa_u32x4* const kd = &s_k[buf][key * kKU];
           pa_u32x4* const vd = &s_v[buf][key * kVU];
-          pa_u32x4 k2[2], v2[2];
+          pa_u32x4 k2[kW], v2[kW];
           if constexpr (kF8) {
-            const float ks = scaled ? __uint_as_float((sc[i] & 255u) << 23) : 1.0f;
-            const float vs = scaled ? __uint_as_float((sc[i] >> 8) << 23) : 1.0f;
-            decode16<kT>(kq[i], ks, k2[0], k2[1]);
-            decode16<kT>(vq[i], vs, v2[0], v2[1]);
+            const uint32_t b2 = scaled ? sc[i] : 0x7f7fu;
+            decode16<kT>(kq[i], __uint_as_float((b2 & 255u) << 23), k2[0], k2[1]);
+            decode16<kT>(vq[i], __uint_as_float((b2 >> 8) << 23), v2[0], v2[1]);
           } else {
             k2[0] = kq[i];
             v2[0] = vq[i];
           }
+          if (part || !whole) {
+            const bool in = (ok >> i) & 1;
 #pragma unroll
-          for (int h = 0; h < (kF8 ? 2 : 1); ++h) {
-            if (!in) v2[h] = pa_u32x4{0, 0, 0, 0};
-            if (part && not_finite<kT>(v2[h])) {
-              v2[h] = pa_u32x4{0, 0, 0, 0};
-              odd_rows |= 1u << i;
+            for (int h = 0; h < kW; ++h) {
+              const bool nf = in && part && not_finite<kT>(v2[h]);
+              odd_rows |= nf ? 1u << i : 0u;
+              const uint32_t z = in && !nf ? 0xffffffffu : 0u;
+              v2[h] &= pa_u32x4{z, z, z, z};
             }
-            const int u = (kF8 ? 2 : 1) * ld_ch + h;
+          }
+#pragma unroll
+          for (int h = 0; h < kW; ++h) {
+            const int u = kW * ld_ch + h;
             kd[u ^ (key & kSwz)] = k2[h];
             vd[u] = v2[h];
           }
         }
         // the wave's keys: 64 / kRowCh of each pass
         uint64_t bad = 0, odd = 0;
-        if (!__all(ok == (1u << kLd) - 1u) || (part && __any(odd_rows))) {
+        if (!whole || (part && __any(odd_rows))) {
 #pragma unroll
           for (int i = 0; i < kLd; ++i) {
             const uint64_t no = __ballot(((ok >> i) & 1) == 0), od = __ballot((odd_rows >> i) & 1);
@@ -717,12 +767,25 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
 #pragma unroll
         for (int sub = 0; sub < kSub; ++sub) {
           const int kb0 = base + 32 * sub;
-          if (kb0 + 32 <= any_lo || kb0 >= min(any_hi, t.khi)) continue;
+          if (kb0 + 32 <= any_lo || kb0 >= any_hi) continue;
           const pa_u32x4 bw = s_bad[buf][sub];
+          // the operands of both products, read ahead of their use where they fit
+          const pa_u32x4* const kt = &s_k[buf][32 * sub * kKU];
+          const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][32 * sub * kVU]) + rd_v;
+          auto read_k = [&](int s, int i) { return kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))]; };
+          auto read_v = [&](int dt) { return join(read_tr(vt + 16 * dt), read_tr(vt + 16 * kVU * 8 + 16 * dt)); };
+          pa_u32x4 va[kAhead ? kDT : 1];
+          pa_u32x4 ka[kAhead ? kS : 1][2];
+          if constexpr (kAhead) {
+#pragma unroll
+            for (int s = 0; s < kS; ++s)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) ka[s][i] = read_k(s, i);
+#pragma unroll
+            for (int dt = 0; dt < kDT; ++dt) va[dt] = read_v(dt);
+          }
           const uint32_t bad = __builtin_amdgcn_readfirstlane(bw.x | bw.y | bw.z | bw.w);
           const bool masked = kb0 < all_lo || kb0 + 32 > all_hi || bad != 0;
-          const pa_u32x4* const kt = &s_k[buf][32 * sub * kKU];
-          const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][32 * sub * kVU]);
           f32x4 s4[kPer][2];
 #pragma unroll
           for (int c = 0; c < kPer; ++c)
@@ -732,25 +795,27 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
           for (int s = 0; s < kS; ++s)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const pa_u32x4 a = kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))];
+              const pa_u32x4 a = kAhead ? ka[kAhead ? s : 0][i] : read_k(s, i);
 #pragma unroll
               for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
             }
-          float f[kPer][8];
-    #pragma unroll
-          for (int c = 0; c < kPer; ++c) {
-            if (p.cap_out != 0.0f) cap_scores(s4[c], p.cap_in, p.cap_out);
-                if (masked) {
-              mask_scores(s4[c], seen_keys(kb0, lc[c].lo, min(lc[c].hi, t.khi), bad, quad));
-            }
-            weigh(s4[c], scale, st[c], acc[c], f[c]);
+          if (p.cap_out != 0.0f) {
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) cap_scores(s4[c], p.cap_in, p.cap_out);
           }
+          if (masked) {
+#pragma unroll
+            for (int c = 0; c < kPer; ++c)
+              mask_scores(s4[c], seen_keys(kb0, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad, quad));
+          }
+          float f[kPer][8];
+          weigh(s4, scale, st, far, acc, f);
           pa_u32x4 pb[kPer];
 #pragma unroll
           for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
 #pragma unroll
           for (int dt = 0; dt < kDT; ++dt) {
-            const pa_u32x4 a = join(read_tr(vt + rd_v + 16 * dt), read_tr(vt + rd_v + 16 * kVU * 8 + 16 * dt));
+            const pa_u32x4 a = kAhead ? va[kAhead ? dt : 0] : read_v(dt);
 #pragma unroll
             for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
           }
@@ -758,36 +823,40 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
       }
     }
     if (!live) continue;
+    PagedArgs& e = fresh_args();
     for (int i = 0; i < n_part; ++i)
 #pragma unroll 1
       for (int h = 0; h < kSub; ++h) {
         const pa_u32x4 o = s_odd[i][h];
         const int first = __builtin_amdgcn_readfirstlane(s_odd_at[i]) + 32 * h;
         for (uint32_t left = __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w); left != 0; left &= left - 1)
-          add_key<D, kPer, false>(p, t, first + __builtin_ctz(left), q, lc, st, acc, quad);
+          add_key<D, kPer, false>(e, t, first + __builtin_ctz(left), q, pos, st, acc, quad);
       }
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       const float l = quad_sum(st[c].l);
-      if (!lc[c].ok) continue;
-      const float m = st[c].m * scale;
+      const int cc = 16 * (kPer * wave + c) + col;
+      if (cc >= t.nc) continue;
+      const float m = st[c].m * e.q_scale;
       if (run.whole) {
-        const int64_t at = static_cast<int64_t>(t.q0 + lc[c].row) * p.Hq + t.hkv * p.G + lc[c].head;
-        const float inv = l == 0.0f ? 0.0f : p.v_scale / l;
-        uint16_t* o = p.out + at * D + 4 * quad;
+        int row, head;
+        lane_column(e, t, cc, row, head);
+        const int64_t at = static_cast<int64_t>(t.q0 + row) * e.Hq + t.hkv * e.G + head;
+        const float inv = l == 0.0f ? 0.0f : e.v_scale / l;
+        uint16_t* o = e.out + at * D + 4 * quad;
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt)
           *reinterpret_cast<pa_u32x2*>(o + 16 * dt) = pa_u32x2{E::pack2(acc[c][dt][0] * inv, acc[c][dt][1] * inv),
                                                               E::pack2(acc[c][dt][2] * inv, acc[c][dt][3] * inv)};
-        if (quad == 0) p.lse[at] = l == 0.0f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+        if (quad == 0) e.lse[at] = l == 0.0f ? -INFINITY : (m + fast_log2(l)) * kLn2;
       } else {
-        const int64_t at = static_cast<int64_t>(run.slot) * (64 * kPer) + 16 * (kPer * wave + c) + col;
-        float* o = p.part_o + at * D + 4 * quad;
+        const int64_t at = static_cast<int64_t>(run.slot) * (64 * kPer) + cc;
+        float* o = e.part_o + at * D + 4 * quad;
 #pragma unroll
         for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<f32x4*>(o + 16 * dt) = acc[c][dt];
         if (quad == 0) {
-          p.part_ml[at * 2] = m;
-          p.part_ml[at * 2 + 1] = l;
+          e.part_ml[at * 2] = m;
+          e.part_ml[at * 2 + 1] = l;
         }
       }
     }
@@ -800,7 +869,8 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams p) {
 // workgroups shared.  One workgroup per (row, query head); the waves take every
 // fourth piece, four loads ahead.  Rows of whole tasks return at once.
 template <int D>
-__global__ void __launch_bounds__(256) combine_kernel(PagedParams p, int kc) {
+__global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
+  PagedArgs& p = fresh_args();
   constexpr int kV = D / 64;  // floats per lane
   __shared__ int s_b;
   __shared__ float s_o[4][D], s_m[4], s_l[4];
