@@ -52,7 +52,7 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int G = Hq / c.Hkv;
   const int64_t cols = (total_q + B - 1) / B * G;  // columns of a request of average length
   ch.body = cols <= 16 ? kBodyStream16 : (cols <= 32 ? kBodyStream32 : (cols <= 64 ? kBodyTile64 : kBodyTile128));
-  if (c.D > 128) ch.body = std::max<int>(ch.body, kBodyTile64);  // (two blocks of such rows and the states exceed a wave's registers)
+  if (c.D > 128) ch.body = kBodyTile64;  // (the only one whose states and operands of 256 dims fit a wave's registers)
   const int room = kBodyCols[ch.body];
   ch.cols = G <= room ? room / G * G : room;  // whole rows where a row's heads fit
   ch.task_rows = G <= room ? ch.cols / G : 2;

@@ -64,20 +64,24 @@ __device__ __forceinline__ Column fresh_column() { return Column{-INFINITY, -INF
 // instead of one fma.
 constexpr float kFar = 1048576.0f;
 
-// Scores of 32 keys (s[c][t][r]: key 16 t + 4 quad + r) to weights in f, moving
+// Scores of 16 kKt keys (s[c][t][r]: key 16 t + 4 quad + r) to weights in f, moving
 // the reference points where a score exceeds one by 2^8 (lazily: p <= 2^8 is as
 // exact, and most blocks rescale nothing).  Called by whole waves; far: some
 // reference point of the wave is.  One branch each for all of the wave's columns:
 // the exponentials share a basic block with the products around them.
-template <int kPer, int kDT>
-__device__ __forceinline__ void weigh(const f32x4 (&s)[kPer][2], float scale, Column (&st)[kPer], bool& far,
-                                      f32x4 (&acc)[kPer][kDT], float (&f)[kPer][8]) {
+template <int kPer, int kKt, int kDT>
+__device__ __forceinline__ void weigh(const f32x4 (&s)[kPer][kKt], float scale, Column (&st)[kPer], bool& far,
+                                      f32x4 (&acc)[kPer][kDT], float (&f)[kPer][4 * kKt]) {
   float top[kPer];
   bool past = false;
 #pragma unroll
   for (int c = 0; c < kPer; ++c) {
-    const float sv[8] = {s[c][0][0], s[c][0][1], s[c][0][2], s[c][0][3], s[c][1][0], s[c][1][1], s[c][1][2], s[c][1][3]};
-    top[c] = max8_nonan(sv);
+    top[c] = s[c][0][0];
+#pragma unroll
+    for (int e = 1; e < 4 * kKt; e += 2) {
+      const float a = s[c][e >> 2][e & 3], b = e + 1 < 4 * kKt ? s[c][(e + 1) >> 2][(e + 1) & 3] : a;
+      top[c] = max3_nonan(top[c], a, b);
+    }
     past = past || top[c] * scale > st[c].past;
   }
   if (__any(past)) {
@@ -100,28 +104,28 @@ __device__ __forceinline__ void weigh(const f32x4 (&s)[kPer][2], float scale, Co
 #pragma unroll
     for (int c = 0; c < kPer; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[c][e] = (st[c].m == -INFINITY ? s[c][e >> 2][e & 3] : s[c][e >> 2][e & 3] - st[c].m) * scale;
+      for (int e = 0; e < 4 * kKt; ++e) f[c][e] = (st[c].m == -INFINITY ? s[c][e >> 2][e & 3] : s[c][e >> 2][e & 3] - st[c].m) * scale;
   } else {
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
       const float mo = st[c].m == -INFINITY ? 0.0f : -st[c].m * scale;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[c][e] = fmaf(s[c][e >> 2][e & 3], scale, mo);
+      for (int e = 0; e < 4 * kKt; ++e) f[c][e] = fmaf(s[c][e >> 2][e & 3], scale, mo);
     }
   }
 #pragma unroll
   for (int c = 0; c < kPer; ++c) {
-    float sum = 0.0f;
+    float sum[2] = {0.0f, 0.0f};  // (two chains)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4 * kKt; ++e) {
       f[c][e] = fast_exp2(f[c][e]);
-      sum = e == 0 ? f[c][e] : sum + f[c][e];
+      sum[e & 1] = e < 2 ? f[c][e] : sum[e & 1] + f[c][e];
     }
-    st[c].l += sum;
+    st[c].l += sum[0] + sum[1];
   }
 }
 
-__device__ __forceinline__ pa_u32x4 pack8(const float (&f)[8]) {
+__device__ __forceinline__ pa_u32x4 pack8(const float* f) {
   return pa_u32x4{E::pack2(f[0], f[1]), E::pack2(f[2], f[3]), E::pack2(f[4], f[5]), E::pack2(f[6], f[7])};
 }
 
@@ -130,9 +134,10 @@ __device__ __forceinline__ pa_u32x4 pack8(const float (&f)[8]) {
 __device__ __forceinline__ float capped(float x, float cap_in, float cap_out) {
   return cap_out * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + fast_exp2(x * cap_in)));
 }
-__device__ __forceinline__ void cap_scores(f32x4 (&c)[2], float cap_in, float cap_out) {
+template <int kKt>
+__device__ __forceinline__ void cap_scores(f32x4 (&c)[kKt], float cap_in, float cap_out) {
 #pragma unroll
-  for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < kKt; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r) c[t][r] = capped(c[t][r], cap_in, cap_out);
 }
@@ -144,7 +149,8 @@ __device__ __forceinline__ uint32_t seen_keys(int base, int lo, int hi, uint32_t
   const uint64_t range = ((1ull << z) - 1) & ~((1ull << a) - 1);
   return (static_cast<uint32_t>(range) & ~bad) >> (4 * quad);
 }
-__device__ __forceinline__ void mask_scores(f32x4 (&c)[2], uint32_t seen) {
+// Masks the scores c[0], c[1] of 32 keys.
+__device__ __forceinline__ void mask_scores(f32x4* c, uint32_t seen) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -289,6 +295,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   constexpr int kVU = D / 8 + 2;            // 16-byte units per staged V row
   constexpr int kDT = D / 16;
   constexpr int kC = 16 * kPer;
+  constexpr int kSets = 1;  // blocks in flight (two, of 8-bit rows: 643 us where one takes 595)
   constexpr int kOut = D + 4;               // floats per column of the joined state
   extern __shared__ int s_pre[];
   __shared__ int s_tmp[4];
@@ -349,25 +356,28 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
     const char* const kb = p.k + at64(t.hkv, p.kv_hs) + 16 * ld_ch;
     const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
-    // the block in flight: rows, scale bytes of key lane % 32, keys without a row
-    pa_u32x4 kq[kNI], vq[kNI];
-    uint32_t sc_next = 0x7f7fu, bad_next = 0;
+    // the blocks in flight
+    struct Flight {
+      pa_u32x4 k[kNI], v[kNI];
+      uint32_t sc, bad;  // scale bytes of key lane % 32, keys without a row
+    };
+    Flight flight[kSets];
     auto entry = [&](int base) {
       return t.table[static_cast<uint32_t>(min((base + (lane & 31)) >> page_shift, last_entry))];
     };
-    auto load = [&](int base, int e) {
+    auto load = [&](int base, int e, Flight& fl) {
       const int key = base + (lane & 31);
       const bool ok = key < t.khi && static_cast<uint32_t>(e) < num_pages;
-      bad_next = ~static_cast<uint32_t>(__ballot(ok));
+      fl.bad = ~static_cast<uint32_t>(__ballot(ok));
       const uint32_t page = ok ? e : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int src = kRI * i + ld_row;
         const char* at = kb + at64(__shfl(page, src), kv_ps) + at64((base + src) & slot_mask, kv_ss);
-        kq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at));
-        vq[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at + v_minus_k));
+        fl.k[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at));
+        fl.v[i] = __builtin_nontemporal_load(reinterpret_cast<const pa_u32x4*>(at + v_minus_k));
       }
-      if constexpr (kF8) sc_next = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
+      if constexpr (kF8) fl.sc = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
     };
 
     Column st[kPer];
@@ -381,25 +391,30 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
 
     bool far = false;
     int n_odd = 0;  // blocks in s_odd
-    // the wave's blocks: every fourth of the run's
+    // the wave's blocks: every fourth of the run's.  Blocks past it are loaded
+    // too (the cache's first page): behind a branch their number would be unknown
+    // to the waits for the blocks before them.
     int base = t.klo + 32 * wave;
-    int e1 = 0;
+    int e_next = 0;  // entries of the block to load next
     if (base < t.khi) {
-      const int e0 = entry(base);
-      e1 = entry(base + 128);
-      load(base, e0);
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        const int e = entry(base + 128 * i);
+        if (i == kSets - 1) e_next = entry(base + 128 * kSets);
+        load(base + 128 * i, e, flight[i]);
+      }
     }
-    for (; base < t.khi; base += 128) {
-      const uint32_t bad = __builtin_amdgcn_readfirstlane(bad_next);
+    auto step = [&](Flight& fl) {
+      const uint32_t bad = __builtin_amdgcn_readfirstlane(fl.bad);
       const bool part = base < all_lo || base + 32 > all_hi;  // some row of the task does not see some key
       const bool masked = part || bad != 0;
-      const uint32_t sc = kF8 && scaled ? sc_next : 0x7f7fu;
+      const uint32_t sc = kF8 && scaled ? fl.sc : 0x7f7fu;
       // rows to LDS
       pa_u32x4 w[kNI][kW];
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
-        if constexpr (kF8) decode16<kT>(vq[i], __uint_as_float((__shfl(sc, kRI * i + ld_row) >> 8) << 23), w[i][0], w[i][1]);
-        else w[i][0] = vq[i];
+        if constexpr (kF8) decode16<kT>(fl.v[i], __uint_as_float((__shfl(sc, kRI * i + ld_row) >> 8) << 23), w[i][0], w[i][1]);
+        else w[i][0] = fl.v[i];
       }
       uint32_t odd = 0;  // keys with V that is not finite
       if (masked) {
@@ -425,15 +440,16 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
 #pragma unroll
       for (int i = 0; i < kNI; ++i) {
         const int r = kRI * i + ld_row;
-        s_k[wave][r * kRL + (ld_ch ^ swizzle(r))] = kq[i];
+        s_k[wave][r * kRL + (ld_ch ^ swizzle(r))] = fl.k[i];
 #pragma unroll
         for (int h = 0; h < kW; ++h) s_v[wave][r * kVU + kW * ld_ch + h] = w[i][h];
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_sched_barrier(0);
-      if (base + 128 < t.khi) {
-        load(base + 128, e1);
-        e1 = entry(base + 256);
+      if (kSets > 1 || base + 128 * kSets < t.khi) {
+        const int e_after = entry(base + 128 * (kSets + 1));  // (ahead of the rows: the wait for it is no wait for them)
+        load(base + 128 * kSets, e_next, fl);
+        e_next = e_after;
       }
       __builtin_amdgcn_sched_barrier(0);
       if (odd != 0) {
@@ -474,7 +490,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       if (masked) {
 #pragma unroll
         for (int c = 0; c < kPer; ++c)
-          mask_scores(s4[c], seen_keys(base, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad | odd, quad));
+          mask_scores(&s4[c][0], seen_keys(base, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad | odd, quad));
       }
       float f[kPer][8];
       weigh(s4, scale, st, far, acc, f);
@@ -486,6 +502,15 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
         const pa_u32x4 a = join(read_tr(vr + 16 * dt), read_tr(vr + 16 * kVU * 8 + 16 * dt));
 #pragma unroll
         for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
+      }
+    };
+    while (base < t.khi) {
+      step(flight[0]);
+      base += 128;
+      if constexpr (kSets > 1) {
+        if (base >= t.khi) break;
+        step(flight[1]);
+        base += 128;
       }
     }
 
@@ -582,7 +607,11 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
   constexpr int kLd = kBlk / kStep;
   constexpr int kSub = kBlk / 32;
   constexpr int kW = kF8 ? 2 : 1;  // staged vectors per chunk
-  constexpr bool kAhead = D <= 128;  // (operands of 256 dims would take 128 registers)
+  // blocks in flight.  64 columns are for calls that the bytes of K and V bound: a
+  // second block where one has 16 KiB (32 requests of 5 rows of 8 heads over 16K 8-bit
+  // keys of 128 dims 182 -> 158 us, over 26K 16-bit ones of 64 dims 207 -> 192), not
+  // where it has 32 (235 -> 243) or rows of 64 bytes, half of a memory line (151 -> 175)
+  constexpr int kSets = kPer == 1 && D * (kF8 ? 1 : 2) == 128 ? 2 : 1;
   static_assert(kLd >= 1, "a block is at least one pass");
   // blocks in which some row of the task misses some key: at either end of its
   // keys the rows' 64 kPer - 1 and one block's
@@ -654,27 +683,31 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
     const char* const kb = p.k + at64(t.hkv, p.kv_hs) + 16 * ld_ch;
     const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
-    int en[kLd];
-    pa_u32x4 kq[kLd], vq[kLd];
-    uint32_t sc[kLd];
-    uint32_t ok = 0;  // bit i: key i of the thread's has a row
-    auto entries = [&](int base) {
+    // the blocks in flight
+    struct Flight {
+      pa_u32x4 k[kLd], v[kLd];
+      uint32_t sc[kLd];
+      uint32_t ok;  // bit i: key i of the thread's has a row
+    };
+    Flight flight[kSets];
+    int en[kLd], en_after[kLd];  // entries of the block to load next, and of the one after
+    auto entries = [&](int base, int (&en)[kLd]) {
 #pragma unroll
       for (int i = 0; i < kLd; ++i)
         en[i] = t.table[static_cast<uint32_t>(min((base + ld_key + kStep * i) >> page_shift, last_entry))];
     };
-    auto load = [&](int base) {
-      ok = 0;
+    auto load = [&](int base, const int (&en)[kLd], Flight& fl) {
+      fl.ok = 0;
 #pragma unroll
       for (int i = 0; i < kLd; ++i) {
         const int key = base + ld_key + kStep * i;
         const bool in = key < t.khi && static_cast<uint32_t>(en[i]) < num_pages;
-        ok |= in ? 1u << i : 0u;
+        fl.ok |= in ? 1u << i : 0u;
         const uint32_t page = in ? en[i] : 0;  // (a key without a row reads page 0: its weight is 0, its V zeroed)
         const char* at = kb + at64(page, kv_ps) + at64(key & slot_mask, kv_ss);
-        kq[i] = *reinterpret_cast<const pa_u32x4*>(at);
-        vq[i] = *reinterpret_cast<const pa_u32x4*>(at + v_minus_k);
-        if constexpr (kF8) sc[i] = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
+        fl.k[i] = *reinterpret_cast<const pa_u32x4*>(at);
+        fl.v[i] = *reinterpret_cast<const pa_u32x4*>(at + v_minus_k);
+        if constexpr (kF8) fl.sc[i] = scales[static_cast<uint64_t>(page) * sc_ps + (scaled ? key & slot_mask : 0)];
       }
     };
 
@@ -689,20 +722,24 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
 
     const int nblk = t.khi > t.klo ? ceil_div(t.khi - t.klo, kBlk) : 0;
     if (nblk > 0) {
-      entries(t.klo);
-      load(t.klo);
-      entries(t.klo + kBlk);
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        entries(t.klo + kBlk * i, en);
+        if (i == kSets - 1) entries(t.klo + kBlk * kSets, en_after);
+        load(t.klo + kBlk * i, en, flight[i]);
+      }
     }
     int n_part = 0;
     bool far = false;
     __syncthreads();  // the run before is done with the tiles
-    for (int bi = 0; bi < nblk; ++bi) {
+    int bi = 0;
+    auto step = [&](Flight& fl) {
       const int buf = bi & 1;
       const int base = t.klo + bi * kBlk;
       const bool part = base < task_lo || base + kBlk > task_hi;
       {
         uint32_t odd_rows = 0;  // bit i: the thread's part of row i
-        const bool whole = __all(ok == (1u << kLd) - 1u);
+        const bool whole = __all(fl.ok == (1u << kLd) - 1u);
 #pragma unroll
         for (int i = 0; i < kLd; ++i) {
           const int key = ld_key + kStep * i;
@@ -710,15 +747,15 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
           pa_u32x4* const vd = &s_v[buf][key * kVU];
           pa_u32x4 k2[kW], v2[kW];
           if constexpr (kF8) {
-            const uint32_t b2 = scaled ? sc[i] : 0x7f7fu;
-            decode16<kT>(kq[i], __uint_as_float((b2 & 255u) << 23), k2[0], k2[1]);
-            decode16<kT>(vq[i], __uint_as_float((b2 >> 8) << 23), v2[0], v2[1]);
+            const uint32_t b2 = scaled ? fl.sc[i] : 0x7f7fu;
+            decode16<kT>(fl.k[i], __uint_as_float((b2 & 255u) << 23), k2[0], k2[1]);
+            decode16<kT>(fl.v[i], __uint_as_float((b2 >> 8) << 23), v2[0], v2[1]);
           } else {
-            k2[0] = kq[i];
-            v2[0] = vq[i];
+            k2[0] = fl.k[i];
+            v2[0] = fl.v[i];
           }
           if (part || !whole) {
-            const bool in = (ok >> i) & 1;
+            const bool in = (fl.ok >> i) & 1;
 #pragma unroll
             for (int h = 0; h < kW; ++h) {
               const bool nf = in && part && not_finite<kT>(v2[h]);
@@ -739,7 +776,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
         if (!whole || (part && __any(odd_rows))) {
 #pragma unroll
           for (int i = 0; i < kLd; ++i) {
-            const uint64_t no = __ballot(((ok >> i) & 1) == 0), od = __ballot((odd_rows >> i) & 1);
+            const uint64_t no = __ballot(((fl.ok >> i) & 1) == 0), od = __ballot((odd_rows >> i) & 1);
 #pragma unroll
             for (int r = 0; r < 64 / kRowCh; ++r) {
               const int key = kStep * i + (64 / kRowCh) * wave + r;
@@ -759,67 +796,80 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
         if (part) ++n_part;
       }
       __syncthreads();  // the block is visible; every wave is done with the block before last
-      if (bi + 1 < nblk) {
-        load(base + kBlk);
-        entries(base + 2 * kBlk);
+      // (with two in flight, blocks past the run are loaded too, the cache's first
+      // page: behind a branch their number would be unknown to the waits for the
+      // one before)
+      if (kSets > 1 || bi + 1 < nblk) {
+#pragma unroll
+        for (int i = 0; i < kLd; ++i) en[i] = en_after[i];
+        entries(base + kBlk * (kSets + 1), en_after);  // (ahead of the rows: the wait for them is no wait for those)
+        load(base + kBlk * kSets, en, fl);
       }
-      if (live) {
+      if (!live || base + kBlk <= any_lo || base >= any_hi) return;
+      // both products take all of the block's keys, so that one vote and one set
+      // of branches serves them and the exponentials of one half overlap the other's
+      // products
+      uint32_t bad[kSub];
+      bool masked = base < all_lo || base + kBlk > all_hi;
+      const pa_u32x4* const kt = &s_k[buf][col * kKU];
+      const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][0]) + rd_v;
+      pa_u32x4 bw[kSub];
 #pragma unroll
-        for (int sub = 0; sub < kSub; ++sub) {
-          const int kb0 = base + 32 * sub;
-          if (kb0 + 32 <= any_lo || kb0 >= any_hi) continue;
-          const pa_u32x4 bw = s_bad[buf][sub];
-          // the operands of both products, read ahead of their use where they fit
-          const pa_u32x4* const kt = &s_k[buf][32 * sub * kKU];
-          const uint16_t* const vt = reinterpret_cast<const uint16_t*>(&s_v[buf][32 * sub * kVU]) + rd_v;
-          auto read_k = [&](int s, int i) { return kt[(16 * i + col) * kKU + ((4 * s + quad) ^ (col & kSwz))]; };
-          auto read_v = [&](int dt) { return join(read_tr(vt + 16 * dt), read_tr(vt + 16 * kVU * 8 + 16 * dt)); };
-          pa_u32x4 va[kAhead ? kDT : 1];
-          pa_u32x4 ka[kAhead ? kS : 1][2];
-          if constexpr (kAhead) {
+      for (int h = 0; h < kSub; ++h) bw[h] = s_bad[buf][h];
+      f32x4 s4[kPer][2 * kSub];
 #pragma unroll
-            for (int s = 0; s < kS; ++s)
+      for (int c = 0; c < kPer; ++c)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) ka[s][i] = read_k(s, i);
+        for (int i = 0; i < 2 * kSub; ++i) s4[c][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int dt = 0; dt < kDT; ++dt) va[dt] = read_v(dt);
+      for (int h = 0; h < kSub; ++h)
+#pragma unroll
+        for (int s = 0; s < kS; ++s)
+#pragma unroll
+          for (int i = 2 * h; i < 2 * h + 2; ++i) {
+            const pa_u32x4 a = kt[16 * i * kKU + ((4 * s + quad) ^ (col & kSwz))];
+#pragma unroll
+            for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
           }
-          const uint32_t bad = __builtin_amdgcn_readfirstlane(bw.x | bw.y | bw.z | bw.w);
-          const bool masked = kb0 < all_lo || kb0 + 32 > all_hi || bad != 0;
-          f32x4 s4[kPer][2];
 #pragma unroll
-          for (int c = 0; c < kPer; ++c)
+      for (int h = 0; h < kSub; ++h) {
+        bad[h] = __builtin_amdgcn_readfirstlane(bw[h].x | bw[h].y | bw[h].z | bw[h].w);
+        masked = masked || bad[h] != 0;
+      }
+      if (p.cap_out != 0.0f) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) s4[c][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c < kPer; ++c) cap_scores(s4[c], p.cap_in, p.cap_out);
+      }
+      if (masked) {
 #pragma unroll
-          for (int s = 0; s < kS; ++s)
+        for (int c = 0; c < kPer; ++c)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const pa_u32x4 a = kAhead ? ka[kAhead ? s : 0][i] : read_k(s, i);
+          for (int h = 0; h < kSub; ++h)
+            mask_scores(&s4[c][2 * h], seen_keys(base + 32 * h, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad[h], quad));
+      }
+      float f[kPer][8 * kSub];
+      weigh(s4, scale, st, far, acc, f);
 #pragma unroll
-              for (int c = 0; c < kPer; ++c) s4[c][i] = E::mfma(a, q[c][s], s4[c][i]);
-            }
-          if (p.cap_out != 0.0f) {
+      for (int h = 0; h < kSub; ++h) {
+        pa_u32x4 pb[kPer];
 #pragma unroll
-            for (int c = 0; c < kPer; ++c) cap_scores(s4[c], p.cap_in, p.cap_out);
-          }
-          if (masked) {
+        for (int c = 0; c < kPer; ++c) pb[c] = pack8(&f[c][8 * h]);
 #pragma unroll
-            for (int c = 0; c < kPer; ++c)
-              mask_scores(s4[c], seen_keys(kb0, first_key(pos[c], window), min(pos[c] + 1, t.khi), bad, quad));
-          }
-          float f[kPer][8];
-          weigh(s4, scale, st, far, acc, f);
-          pa_u32x4 pb[kPer];
+        for (int dt = 0; dt < kDT; ++dt) {
+          const uint16_t* const at = vt + 32 * h * kVU * 8 + 16 * dt;
+          const pa_u32x4 a = join(read_tr(at), read_tr(at + 16 * kVU * 8));
 #pragma unroll
-          for (int c = 0; c < kPer; ++c) pb[c] = pack8(f[c]);
-#pragma unroll
-          for (int dt = 0; dt < kDT; ++dt) {
-            const pa_u32x4 a = kAhead ? va[kAhead ? dt : 0] : read_v(dt);
-#pragma unroll
-            for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
-          }
+          for (int c = 0; c < kPer; ++c) acc[c][dt] = E::mfma(a, pb[c], acc[c][dt]);
         }
+      }
+    };
+    while (bi < nblk) {
+      step(flight[0]);
+      ++bi;
+      if constexpr (kSets > 1) {
+        if (bi >= nblk) break;
+        step(flight[1]);
+        ++bi;
       }
     }
     if (!live) continue;
@@ -959,16 +1009,15 @@ typedef void (*Kernel)(PagedParams);
 
 template <int D>
 Kernel body_kernel(int body) {
-  constexpr int kBlk = D > 128 ? 32 : 64;
-  switch (body) {
-    case kBodyStream16:
-      if constexpr (D <= 128) return stream_kernel<D, 1>;
-      return nullptr;
-    case kBodyStream32:
-      if constexpr (D <= 128) return stream_kernel<D, 2>;
-      return nullptr;
-    case kBodyTile64: return tile_kernel<D, 1, kBlk, 2>;
-    default: return tile_kernel<D, 2, kBlk, (D > 128 ? 1 : 2)>;
+  if constexpr (D <= 128) {
+    switch (body) {
+      case kBodyStream16: return stream_kernel<D, 1>;
+      case kBodyStream32: return stream_kernel<D, 2>;
+      case kBodyTile64: return tile_kernel<D, 1, 64, 2>;
+      default: return tile_kernel<D, 2, 64, 2>;
+    }
+  } else {
+    return tile_kernel<D, 1, 32, 2>;  // (the other bodies' states and operands of 256 dims exceed a wave's registers)
   }
 }
 Kernel body_of(int D, int body) {
