@@ -27,7 +27,7 @@ bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
 
 struct Choice {
-  int body = 0, cols = 0, task_rows = 0, unit_shift = 0, stream = 0, grid = 0;
+  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = 0, grid = 0;
   size_t plan_bytes = 0, ml_bytes = 0, o_bytes = 0;
   size_t bytes() const { return plan_bytes + ml_bytes + o_bytes; }
 };
@@ -56,9 +56,19 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int room = kBodyCols[ch.body];
   ch.cols = G <= room ? room / G * G : room;  // whole rows where a row's heads fit
   ch.task_rows = G <= room ? ch.cols / G : 2;
+  // The stream body's waves read 256 bytes of a token at a time: two or four heads'
+  // rows where they lie side by side.  8 KV heads of 128 dims, 8-bit, one head / two
+  // (us): 64 requests over 26K keys 645 / 600, 16 over 32K 227 / 211, 4 over 128K 219 /
+  // 199, 64 over 1K 46 / 48; of 64 dims, one / four: 573 / 466, 194 / 148, 164 / 156, 48 /
+  // 41.  Not where few tasks share the keys among many workgroups (fewer, larger
+  // partial states then): 1 request over 128K keys 75 / 80, over 4K 27 / 32.
+  const int64_t row = static_cast<int64_t>(c.D) * (c.cache_dtype == MAC_DTYPE_E4M3 ? 1 : 2);
+  const int64_t head_tasks = std::min<int64_t>(total_q, total_q * G / ch.cols + B) * c.Hkv;
+  if (ch.body <= kBodyStream32 && c.k_head_stride == row && head_tasks >= 32)
+    while (row << ch.heads_shift < 256 && c.Hkv % (2 << ch.heads_shift) == 0) ++ch.heads_shift;
   // bounds on the tasks: of this batch's rows, and of any row offsets (a
   // request's rows lie within total_q)
-  const int64_t tasks = (std::min<int64_t>(total_q, total_q * G / ch.cols + B)) * c.Hkv;
+  const int64_t tasks = (std::min<int64_t>(total_q, total_q * G / ch.cols + B)) * (c.Hkv >> ch.heads_shift);
   const int64_t worst = static_cast<int64_t>(B) * ((total_q * G + ch.cols - 1) / ch.cols) * c.Hkv;
   if (worst >= INT_MAX) return false;
   const int resident = variant(q_dtype, c.cache_dtype).resident(c.D, ch.body, B);
@@ -68,11 +78,11 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
     ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));
     return true;
   }
-  ch.unit_shift = 7;
+  ch.unit_shift = 7 - ch.heads_shift;  // one block of each wave
   while (ch.unit_shift < 30 && (((max_keys + (int64_t{1} << ch.unit_shift) - 1) >> ch.unit_shift) + 1) * worst >= INT_MAX) ++ch.unit_shift;
   if (2 * worst >= INT_MAX || total_q * Hq > INT_MAX) return false;
   ch.plan_bytes = up16(sizeof(int) * (static_cast<size_t>(B) + 1));
-  const size_t slots = 2 * static_cast<size_t>(ch.grid) * room;
+  const size_t slots = 2 * static_cast<size_t>(ch.grid) * (room << ch.heads_shift);
   ch.ml_bytes = slots * 2 * sizeof(float);
   ch.o_bytes = slots * c.D * sizeof(float);
   return true;
@@ -176,6 +186,7 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   // (a window of 2^30 keys or more covers any request's)
   p.window_left = a->window_left < 0 || a->window_left >= (1 << 30) ? -1 : a->window_left;
   p.cols = ch.cols;
+  p.heads_shift = ch.heads_shift;
   p.task_rows = ch.task_rows;
   p.unit_shift = ch.unit_shift;
   p.stream = ch.stream;

@@ -25,8 +25,8 @@ struct PagedParams {
   const int32_t* req_ids;  // row of the table for each request, or NULL: the request's number
   uint16_t* out;
   float* lse;
-  float* part_o;   // stream form: [2 grid][cols][D] unnormalised partial outputs
-  float* part_ml;  // [2 grid][cols][2] their reference points (log2 units) and sums
+  float* part_o;   // stream form: [2 grid][heads][body's columns][D] unnormalised partial outputs
+  float* part_ml;  // [2 grid][heads][columns][2] their reference points (log2 units) and sums
   int32_t* plan;   // [B + 1] units before each request, for the combining launch
   int64_t q_ts, q_hs;                          // elements
   uint32_t kv_ps, kv_ss, kv_hs;  // bytes: page, slot and head strides of K and of V
@@ -36,7 +36,8 @@ struct PagedParams {
   int B, Hq, Hkv, G;
   int table_rows, table_cols, page_shift;
   int window_left;  // < 0: none
-  int cols;         // columns of a task (whole rows where a row's heads fit one)
+  int cols;         // columns of a task per KV head (whole rows where a row's heads fit one)
+  int heads_shift;  // a task takes 2^heads_shift KV heads (stream body)
   int task_rows;    // most rows that a task's columns touch
   int unit_shift;   // stream form; 0 units: plain form
   int stream;       // 1: stream form
@@ -63,7 +64,7 @@ struct PagedRequest {
   int q0, n;    // first row, rows
   int len;      // kv length (row r sits at position len - n + r)
   int keys;     // cached keys that the table can name
-  int tasks;    // column tasks per KV head
+  int tasks;    // column tasks per KV head (or group of 2^heads_shift)
   int units;    // stream form: units per task
 };
 
@@ -84,7 +85,7 @@ __device__ __forceinline__ PagedRequest paged_request(PagedArgs& p, int b) {
 
 // Units (stream form) or tasks (plain form) of a request.
 __device__ __forceinline__ int paged_weight(PagedArgs& p, const PagedRequest& r) {
-  return r.tasks * p.Hkv * (p.stream ? r.units : 1);
+  return r.tasks * (p.Hkv >> p.heads_shift) * (p.stream ? r.units : 1);
 }
 
 // Exclusive prefix of the requests' weights in s_pre[B + 1], by a workgroup of
@@ -147,7 +148,7 @@ __device__ __forceinline__ int stream_owner(int x, int total, int groups) {
 
 // One of a task's runs of keys.
 struct PagedTask {
-  int b, hkv, gc0;      // request, KV head, first column of the request's rows x G
+  int b, hkv, gc0;      // request, (first) KV head, first column of the request's rows x G
   int q0, n, len;       // of the request
   int nc;               // columns
   int row0, row1;       // first and last row
@@ -158,8 +159,9 @@ struct PagedTask {
 __device__ __forceinline__ PagedTask paged_task(PagedArgs& p, int b, const PagedRequest& r, int index) {
   PagedTask t;
   t.b = b;
-  t.hkv = index / r.tasks;
-  const int ct = index - t.hkv * r.tasks;
+  const int group = index / r.tasks;
+  const int ct = index - group * r.tasks;
+  t.hkv = group << p.heads_shift;
   t.q0 = r.q0;
   t.n = r.n;
   t.len = r.len;

@@ -32,6 +32,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "mac_paged_attention.h"
@@ -180,17 +181,17 @@ __device__ __forceinline__ void row8(const char* row, int d, float scale, float 
   x[4] = E::low(w.z); x[5] = E::high(w.z); x[6] = E::low(w.w); x[7] = E::high(w.w);
 }
 
-// Adds one key to the states of the rows that see it, in fp32 on the vector
-// units.  kSplitQ: q's chunks in the order of the 8-bit stream body.
+// Adds one key of KV head hkv to the states of the rows that see it, in fp32 on the
+// vector units.  kSplitQ: q's chunks in the order of the 8-bit stream body.
 template <int D, int kPer, bool kSplitQ>
-__device__ __forceinline__ void add_key(PagedArgs& p, const PagedTask& t, int key, const pa_u32x4 (&q)[kPer][D / 32],
+__device__ __forceinline__ void add_key(PagedArgs& p, const PagedTask& t, int hkv, int key, const pa_u32x4 (&q)[kPer][D / 32],
                                         const int (&pos)[kPer], Column (&st)[kPer], f32x4 (&acc)[kPer][D / 16], int quad) {
   const int page = t.table[key >> p.page_shift];
   const int slot = key & ((1 << p.page_shift) - 1);
-  const uint64_t row = at64(page, p.kv_ps) + at64(slot, p.kv_ss) + at64(t.hkv, p.kv_hs);
+  const uint64_t row = at64(page, p.kv_ps) + at64(slot, p.kv_ss) + at64(hkv, p.kv_hs);
   const char* kr = p.k + row;
   const char* vr = p.v + row;
-  const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((static_cast<int64_t>(page) * p.Hkv + t.hkv) << p.page_shift) + slot] : 0x7f7fu;
+  const uint32_t sc = kF8 && p.scales != nullptr ? p.scales[((static_cast<int64_t>(page) * p.Hkv + hkv) << p.page_shift) + slot] : 0x7f7fu;
   const float ks = __uint_as_float((sc & 255u) << 23), vs = __uint_as_float((sc >> 8) << 23);
   float s[kPer] = {};
 #pragma unroll
@@ -275,7 +276,10 @@ __device__ __forceinline__ bool next_run(PagedArgs& p, const int* s_pre, int x0,
 // ------------------------------------------------------------ stream body ---
 
 // Few columns (16 kPer): the bytes of K and V bound the call, so the four waves
-// take different keys, 32 at a time, and meet once, at the end of a run.  A
+// take different keys, 32 at a time, and meet once, at the end of a run.  Rows of
+// fewer than 256 bytes are read with their neighbours': two (four) waves take two
+// (four) KV heads of the same keys, and a token's heads, which lie side by side,
+// come from memory together (@@).  A
 // wave needs no barrier on its way: it loads whole rows (a quarter of a wave
 // reads one or two of them; operand order, a row per lane, takes eight times the
 // cache lookups per byte and ran at 4.2 TB/s where this runs at @@), and stages
@@ -322,17 +326,22 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   const int ld_row = lane / kRL, ld_ch = lane % kRL;  // the lane's row of a load, its chunk
   const uint16_t* const vr = reinterpret_cast<const uint16_t*>(&s_v[wave][0]) + (4 * quad + (col >> 2)) * (kVU * 8) + 4 * (col & 3);
 
+  // the wave's head in the task and its share of the keys
+  const int heads_shift = a0.heads_shift, heads = 1 << heads_shift;
+  const int own_head = wave & (heads - 1), key_step = 128 >> heads_shift;
+
   int x = x0;
   Run run;
   while (next_run(fresh_args(), s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
     PagedArgs& p = fresh_args();
+    const int hkv = t.hkv + own_head;
     const float scale = p.q_scale;
     const int window = p.window_left;
     // (a static cache loads a word of K in the scale's place: a load that only
     // some calls make would leave the waits behind it uncounted)
     const bool scaled = kF8 && p.scales != nullptr;
-    const uint16_t* const scales = scaled ? p.scales + (t.hkv << p.page_shift) : reinterpret_cast<const uint16_t*>(p.k);
+    const uint16_t* const scales = scaled ? p.scales + (hkv << p.page_shift) : reinterpret_cast<const uint16_t*>(p.k);
     const uint32_t sc_ps = scaled ? static_cast<uint32_t>(p.Hkv) << p.page_shift : 0;  // scale words per page
     const int page_shift = p.page_shift, slot_mask = (1 << p.page_shift) - 1;
     const uint32_t num_pages = p.num_pages, kv_ps = p.kv_ps, kv_ss = p.kv_ss;
@@ -344,7 +353,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       int row, head;
       lane_column(p, t, 16 * c + col, row, head);
       pos[c] = t.len - t.n + row;
-      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + row) * p.q_ts + (t.hkv * p.G + head) * p.q_hs;
+      const uint16_t* at = p.q + static_cast<int64_t>(t.q0 + row) * p.q_ts + (hkv * p.G + head) * p.q_hs;
 #pragma unroll
       for (int s = 0; s < kS; ++s)
         q[c][s] = *reinterpret_cast<const pa_u32x4*>(at + (kF8 ? 64 * (s >> 1) + 16 * quad + 8 * (s & 1) : 32 * s + 8 * quad));
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
     const int all_lo = first_key(t.len - t.n + t.row1, window);
     const int all_hi = t.len - t.n + t.row0 + 1;
 
-    const char* const kb = p.k + at64(t.hkv, p.kv_hs) + 16 * ld_ch;
+    const char* const kb = p.k + at64(hkv, p.kv_hs) + 16 * ld_ch;
     const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
     // the blocks in flight
@@ -391,17 +400,18 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
 
     bool far = false;
     int n_odd = 0;  // blocks in s_odd
-    // the wave's blocks: every fourth of the run's.  Blocks past it are loaded
+    // the wave's blocks: every fourth of the run's (of two
+    // heads: every second).  Blocks past it are loaded
     // too (the cache's first page): behind a branch their number would be unknown
     // to the waits for the blocks before them.
-    int base = t.klo + 32 * wave;
+    int base = t.klo + 32 * (wave >> heads_shift);
     int e_next = 0;  // entries of the block to load next
     if (base < t.khi) {
 #pragma unroll
       for (int i = 0; i < kSets; ++i) {
-        const int e = entry(base + 128 * i);
-        if (i == kSets - 1) e_next = entry(base + 128 * kSets);
-        load(base + 128 * i, e, flight[i]);
+        const int e = entry(base + key_step * i);
+        if (i == kSets - 1) e_next = entry(base + key_step * kSets);
+        load(base + key_step * i, e, flight[i]);
       }
     }
     auto step = [&](Flight& fl) {
@@ -446,9 +456,9 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_sched_barrier(0);
-      if (kSets > 1 || base + 128 * kSets < t.khi) {
-        const int e_after = entry(base + 128 * (kSets + 1));  // (ahead of the rows: the wait for it is no wait for them)
-        load(base + 128 * kSets, e_next, fl);
+      if (kSets > 1 || base + key_step * kSets < t.khi) {
+        const int e_after = entry(base + key_step * (kSets + 1));  // (ahead of the rows: the wait for it is no wait for them)
+        load(base + key_step * kSets, e_next, fl);
         e_next = e_after;
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -506,11 +516,11 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
     };
     while (base < t.khi) {
       step(flight[0]);
-      base += 128;
+      base += key_step;
       if constexpr (kSets > 1) {
         if (base >= t.khi) break;
         step(flight[1]);
-        base += 128;
+        base += key_step;
       }
     }
 
@@ -519,7 +529,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       const pa_u32x2 o = s_odd[wave][i];
       const int first = __builtin_amdgcn_readfirstlane(o.x);
       for (uint32_t left = __builtin_amdgcn_readfirstlane(o.y); left != 0; left &= left - 1)
-        add_key<D, kPer, kF8>(e, t, first + __builtin_ctz(left), q, pos, st, acc, quad);
+        add_key<D, kPer, kF8>(e, t, hkv, first + __builtin_ctz(left), q, pos, st, acc, quad);
     }
 
     // the four waves' states joined
@@ -534,9 +544,8 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
     __syncthreads();
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
-      float m = s_m[0][16 * c + col];
-#pragma unroll
-      for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][16 * c + col]);
+      float m = s_m[own_head][16 * c + col];
+      for (int w = own_head + heads; w < 4; w += heads) m = fmaxf(m, s_m[w][16 * c + col]);
       const float own = s_m[wave][16 * c + col];
       // (-inf for a state without keys: weight 0, or 1 where no wave has any)
       const float f = own == m ? 1.0f : fast_exp2(own - m);
@@ -547,39 +556,38 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       // 16 threads per column, D / 16 dims each
       const int cc = tid >> 4, d0 = (tid & 15) * kDT;
       const int gcol = 16 * c + cc;
-      float mx = s_m[0][gcol], l = 0.0f;
+      for (int h = 0; h < heads; ++h) {
+        float mx = s_m[h][gcol], l = 0.0f;
+        for (int w = h + heads; w < 4; w += heads) mx = fmaxf(mx, s_m[w][gcol]);
+        for (int w = h; w < 4; w += heads) l += s_l[w][gcol] * (s_m[w][gcol] == mx ? 1.0f : fast_exp2(s_m[w][gcol] - mx));
+        if (gcol < t.nc) {
+          float r[kDT];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) mx = fmaxf(mx, s_m[w][gcol]);
+          for (int i = 0; i < kDT; i += 4) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int w = h; w < 4; w += heads) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&s_v[w][0]) + cc * kOut + d0 + i);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) l += s_l[w][gcol] * (s_m[w][gcol] == mx ? 1.0f : fast_exp2(s_m[w][gcol] - mx));
-      if (gcol < t.nc) {
-        float r[kDT];
+            for (int j = 0; j < 4; ++j) r[i + j] = sum[j];
+          }
+          if (run.whole) {
+            int row, head;
+            lane_column(e, t, gcol, row, head);
+            const int64_t at = static_cast<int64_t>(t.q0 + row) * e.Hq + (t.hkv + h) * e.G + head;
+            const float inv = l == 0.0f ? 0.0f : e.v_scale / l;
 #pragma unroll
-        for (int i = 0; i < kDT; i += 4) {
-          f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < kDT; i += 4)
+              *reinterpret_cast<pa_u32x2*>(e.out + at * D + d0 + i) =
+                  pa_u32x2{E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv)};
+            if (d0 == 0) e.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
+          } else {
+            const int64_t at = (static_cast<int64_t>(run.slot) * heads + h) * kC + gcol;
 #pragma unroll
-          for (int w = 0; w < 4; ++w) sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(&s_v[w][0]) + cc * kOut + d0 + i);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) r[i + j] = sum[j];
-        }
-        if (run.whole) {
-          int row, head;
-          lane_column(e, t, gcol, row, head);
-          const int64_t at = static_cast<int64_t>(t.q0 + row) * e.Hq + t.hkv * e.G + head;
-          const float inv = l == 0.0f ? 0.0f : e.v_scale / l;
-#pragma unroll
-          for (int i = 0; i < kDT; i += 4)
-            *reinterpret_cast<pa_u32x2*>(e.out + at * D + d0 + i) =
-                pa_u32x2{E::pack2(r[i] * inv, r[i + 1] * inv), E::pack2(r[i + 2] * inv, r[i + 3] * inv)};
-          if (d0 == 0) e.lse[at] = l == 0.0f ? -INFINITY : (mx + fast_log2(l)) * kLn2;
-        } else {
-          const int64_t at = static_cast<int64_t>(run.slot) * kC + gcol;
-#pragma unroll
-          for (int i = 0; i < kDT; i += 4)
-            *reinterpret_cast<f32x4*>(e.part_o + at * D + d0 + i) = f32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
-          if (d0 == 0) {
-            e.part_ml[at * 2] = mx;
-            e.part_ml[at * 2 + 1] = l;
+            for (int i = 0; i < kDT; i += 4)
+              *reinterpret_cast<f32x4*>(e.part_o + at * D + d0 + i) = f32x4{r[i], r[i + 1], r[i + 2], r[i + 3]};
+            if (d0 == 0) {
+              e.part_ml[at * 2] = mx;
+              e.part_ml[at * 2 + 1] = l;
+            }
           }
         }
       }
@@ -880,7 +888,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
         const pa_u32x4 o = s_odd[i][h];
         const int first = __builtin_amdgcn_readfirstlane(s_odd_at[i]) + 32 * h;
         for (uint32_t left = __builtin_amdgcn_readfirstlane(o.x | o.y | o.z | o.w); left != 0; left &= left - 1)
-          add_key<D, kPer, false>(e, t, first + __builtin_ctz(left), q, pos, st, acc, quad);
+          add_key<D, kPer, false>(e, t, t.hkv, first + __builtin_ctz(left), q, pos, st, acc, quad);
       }
 #pragma unroll
     for (int c = 0; c < kPer; ++c) {
@@ -941,14 +949,15 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   const int hkv = head / p.G;
   const int gc = static_cast<int>(row - r.q0) * p.G + head - hkv * p.G;
   const int ct = gc / p.cols, col = gc - ct * p.cols;
-  const int first = p.plan[b] + (hkv * r.tasks + ct) * r.units;
+  const int group = hkv >> p.heads_shift;
+  const int first = p.plan[b] + (group * r.tasks + ct) * r.units;
   const int wa = stream_owner(first, total, groups), wb = stream_owner(first + r.units - 1, total, groups);
   if (wa == wb) return;  // stored by its workgroup
   const bool at_start = stream_begin(wa, total, groups) == first;
   const int n = wb - wa + 1;
   auto place = [&](int i) {
     const int64_t slot = 2 * static_cast<int64_t>(wa + i) + (i == 0 && !at_start ? 1 : 0);
-    return slot * kc + col;
+    return ((slot << p.heads_shift) + hkv - (group << p.heads_shift)) * kc + col;
   };
   float m = -INFINITY, l = 0.0f, o[kV] = {};
   constexpr int kB = 4;
@@ -1033,12 +1042,23 @@ size_t plan_bytes(int B) { return sizeof(int) * (static_cast<size_t>(B) + 1); }
 namespace mac {
 
 int MAC_PAGED_CAT(paged_resident_, MAC_PAGED_NAME)(int D, int body, int B) {
-  int dev = 0, cus = 256, v = 0, per = 1;
-  if (hipGetDevice(&dev) == hipSuccess && hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0)
-    cus = v;
-  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, reinterpret_cast<const void*>(body_of(D, body)), 256, plan_bytes(B)) != hipSuccess ||
+  // (queries of the runtime, some microseconds each: once per device for plans of
+  // up to 4 KiB, which take a workgroup's room from none of the bodies)
+  constexpr int kDevices = 64;
+  constexpr size_t kPlan = 4096;
+  static std::atomic<int> known[kDevices][3][kBodies];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) return 1;
+  const size_t bytes = std::max(plan_bytes(B), kPlan);
+  std::atomic<int>* slot = bytes == kPlan && dev >= 0 && dev < kDevices ? &known[dev][D == 64 ? 0 : (D == 128 ? 1 : 2)][body] : nullptr;
+  if (slot != nullptr)
+    if (const int n = slot->load(std::memory_order_relaxed)) return n;
+  int cus = 256, v = 0, per = 1;
+  if (hipDeviceGetAttribute(&v, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && v > 0) cus = v;
+  if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, reinterpret_cast<const void*>(body_of(D, body)), 256, bytes) != hipSuccess ||
       per < 1)
     per = 1;
+  if (slot != nullptr) slot->store(cus * per, std::memory_order_relaxed);
   return cus * per;
 }
 

@@ -16,6 +16,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 from functools import lru_cache
 from typing import Any
 
@@ -205,16 +206,16 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _p, _i64, _i64, _i32, _p, _i32, _p, _i32,
         _i64, _i32, _i32, _i32, _i32, _p]
     lib.mac_decode_rope_preserve_q_bf16.restype = ctypes.c_int
-    cache = ctypes.POINTER(MacPagedCache)
-    lib.mac_paged_cache_write_fp8.argtypes = [cache, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i32, _i64, _p]
+    # (argument blocks of these as packed bytes or by reference)
+    lib.mac_paged_cache_write_fp8.argtypes = [_p, _p, _i64, _i64, _p, _i64, _i64, _i32, _p, _i32, _i64, _p]
     lib.mac_paged_cache_write_fp8.restype = ctypes.c_int
-    lib.mac_paged_rope_write_fp8.argtypes = [cache, ctypes.POINTER(MacPagedRopeArgs), _p]
+    lib.mac_paged_rope_write_fp8.argtypes = [_p, _p, _p]
     lib.mac_paged_rope_write_fp8.restype = ctypes.c_int
-    lib.mac_paged_cache_read_fp8.argtypes = [cache, _p, _i32, _i64, _p, _p, _i32, _p]
+    lib.mac_paged_cache_read_fp8.argtypes = [_p, _p, _i32, _i64, _p, _p, _i32, _p]
     lib.mac_paged_cache_read_fp8.restype = ctypes.c_int
-    lib.mac_paged_chunk_attention_workspace.argtypes = [cache, ctypes.POINTER(MacPagedAttentionArgs)]
+    lib.mac_paged_chunk_attention_workspace.argtypes = [_p, _p]
     lib.mac_paged_chunk_attention_workspace.restype = ctypes.c_int64
-    lib.mac_paged_chunk_attention.argtypes = [cache, ctypes.POINTER(MacPagedAttentionArgs), _p, _i64, _p]
+    lib.mac_paged_chunk_attention.argtypes = [_p, _p, _p, _i64, _p]
     lib.mac_paged_chunk_attention.restype = ctypes.c_int
     if lib.mac_abi_version() != ABI_VERSION:
         raise RuntimeError(
@@ -1012,32 +1013,71 @@ def load_mac_decode_rope_preserve_extension(verbose: bool = False) -> Any:
 # ------------------------------------------------------- paged 8-bit cache ---
 
 _DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
-_CACHE_SIZE = ctypes.sizeof(MacPagedCache)
-_PAGED_ROPE_SIZE = ctypes.sizeof(MacPagedRopeArgs)
-_PAGED_ATTENTION_SIZE = ctypes.sizeof(MacPagedAttentionArgs)
+_E4M3 = torch.float8_e4m3fn
+_HALF_DTYPES = (torch.bfloat16, torch.float16)
 _SCALE_DTYPES = (torch.uint8, torch.float8_e8m0fnu)
+_INDEX_DTYPES = (torch.int32, torch.int64)
+_I32_ONLY = (torch.int32,)
+_ANY_WINDOW = 1 << 30  # a window that covers every key of any request
 
 
-def _check_vector(t: torch.Tensor, name: str, device: torch.device, dtypes: tuple, n: int | None = None) -> None:
+# The calls below are short next to their own marshalling: a decode batch's write
+# takes the GPU 4 us.  So each tensor is looked at by one expression when all is
+# well (get_device() is -1 off the GPU), its message comes from a second look, and
+# the argument blocks are packed in one call instead of field by field (a decode
+# batch's write 13.7 us a call with ctypes structures and a device object per
+# tensor, @W now; a decode step of one request 24.2 and @A).
+
+
+def _packer(cls: type, fmt: str):
+    """struct.pack for a C block, with the layout of its ctypes mirror."""
+    packer = struct.Struct("@" + fmt)
+    size = ctypes.sizeof(cls)
+    assert packer.size <= size < packer.size + 8, (cls, packer.size, size)
+    pad = struct.Struct("@" + fmt + f"{size - packer.size}x").pack
+
+    def pack(*values) -> bytes:
+        try:
+            return pad(*values)
+        except (struct.error, OverflowError, TypeError) as e:
+            raise RuntimeError(f"argument out of range: {e}") from None
+
+    return pack, size
+
+
+_pack_cache, _CACHE_SIZE = _packer(MacPagedCache, "IIPPPqqqqqqqiiiiff")
+_pack_rope, _PAGED_ROPE_SIZE = _packer(MacPagedRopeArgs, "IIPPPqqqqqqPPqqPPqiiiiii")
+_pack_attention, _PAGED_ATTENTION_SIZE = _packer(MacPagedAttentionArgs, "IIPqqPPPqPPPqiiiiiidd")
+
+
+def _check_vector(t: torch.Tensor, name: str, device: int, dtypes: tuple, n: int | None = None) -> None:
     """A contiguous index vector on ``device`` (of n entries)."""
-    if (t.is_cuda and t.dtype in dtypes and t.dim() == 1 and t.is_contiguous() and t.device == device
-            and (n is None or t.shape[0] == n)):
+    if (t.get_device() == device and t.dtype in dtypes and t.dim() == 1 and t.is_contiguous()
+            and (n is None or t.size(0) == n)):
         return
     _check(t.is_cuda, f"{name} must be CUDA")
-    _check(t.device == device, f"{name}: tensors must be on the same device")
+    _check(t.get_device() == device, f"{name}: tensors must be on the same device")
     _check(t.dtype in dtypes, f"{name} has wrong dtype")
     _check(t.dim() == 1, f"{name} has wrong rank")
     _check(t.is_contiguous(), f"{name} must be contiguous")
-    _check(n is None or t.shape[0] == n, f"{name} has wrong length")
+    _check(n is None or t.size(0) == n, f"{name} has wrong length")
 
 
-def _check_rows(t: torch.Tensor, name: str, device: torch.device, heads: int | None, d: int) -> None:
-    """Rows [tokens, heads, D], the last dimension contiguous."""
+def _check_rows(t: torch.Tensor, name: str, device: int, heads: int | None, d: int) -> tuple:
+    """Rows [tokens, heads, D], the last dimension contiguous: their shape and strides."""
+    if t.get_device() == device and t.dtype in _HALF_DTYPES and t.dim() == 3:
+        shape, stride = t.shape, t.stride()
+        if shape[2] == d and stride[2] == 1 and (heads is None or shape[1] == heads):
+            return shape, stride
     _check(t.is_cuda, f"{name} must be CUDA")
-    _check(t.device == device, f"{name}: tensors must be on the same device")
-    _check(t.dtype in (torch.bfloat16, torch.float16), f"{name} must be bfloat16 or float16")
+    _check(t.get_device() == device, f"{name}: tensors must be on the same device")
+    _check(t.dtype in _HALF_DTYPES, f"{name} must be bfloat16 or float16")
     _check(t.dim() == 3 and t.shape[2] == d and (heads is None or t.shape[1] == heads), f"{name} has wrong shape")
-    _check(t.stride(2) == 1, f"{name} must have contiguous last dimension")
+    raise RuntimeError(f"{name} must have contiguous last dimension")
+
+
+def _check_result(t: torch.Tensor, shape: tuple, dtype: torch.dtype, device: int, msg: str) -> None:
+    _check(t.get_device() == device and t.dtype == dtype and t.shape == shape and t.is_contiguous(), msg)
 
 
 class PagedCacheExtension:
@@ -1048,40 +1088,57 @@ class PagedCacheExtension:
     logit caps, other head sizes and larger groups are left to the engine).
 
     Caches: k_cache, v_cache [pages, page_size, Hkv, D], float8_e4m3fn (attention:
-    or q's dtype), any page, slot and head strides of whole 16 bytes, page_size
-    a power of two (a pool [tokens, Hkv, D] is ``pool.unsqueeze(1)``).
-    kv_scales: uint8 or float8_e8m0fnu [pages, Hkv, page_size, 2], a row's K and
-    V scale as E8M0 bytes (2^(byte - 127)), or None: values are codes times the
-    static k_scale / v_scale."""
+    or q's dtype), page, slot and head strides of whole 16 bytes in any order (for
+    attention the same ones in both), page_size a power of two (a pool [tokens,
+    Hkv, D] is ``pool.unsqueeze(1)``).  kv_scales: uint8 or float8_e8m0fnu [pages,
+    Hkv, page_size, 2], a row's K and V scale as E8M0 bytes (2^(byte - 127)), or
+    None: values are codes times the static k_scale / v_scale."""
 
     def __init__(self, lib: ctypes.CDLL):
         self._lib = lib
 
     @staticmethod
-    def _cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only: bool = True) -> MacPagedCache:
-        dt = k_cache.dtype
-        _check(k_cache.is_cuda and v_cache.is_cuda, "k_cache and v_cache must be CUDA")
-        _check(dt == torch.float8_e4m3fn or (not fp8_only and dt in (torch.bfloat16, torch.float16)),
-               "k_cache must be float8_e4m3fn" + ("" if fp8_only else ", bfloat16 or float16"))
-        _check(v_cache.dtype == dt, "v_cache must have k_cache's dtype")
-        _check(k_cache.dim() == 4, "k_cache must be [pages,page_size,Hkv,D]")
-        pages, page, hkv, d = k_cache.shape
-        _check(v_cache.shape == k_cache.shape, "v_cache must match k_cache")
-        _check(v_cache.device == k_cache.device, "v_cache: tensors must be on the same device")
-        ks, vs = k_cache.stride(), v_cache.stride()
-        _check(ks[3] == 1 and vs[3] == 1, "k_cache and v_cache must have contiguous last dimension")
+    def _cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only: bool = True) -> tuple:
+        """(packed block, device, Hkv, D) of a cache."""
+        dt, dev = k_cache.dtype, k_cache.get_device()
+        if not (dev >= 0 and v_cache.get_device() == dev and v_cache.dtype == dt and k_cache.dim() == 4
+                and (dt == _E4M3 or (not fp8_only and dt in _HALF_DTYPES))):
+            _check(k_cache.is_cuda and v_cache.is_cuda, "k_cache and v_cache must be CUDA")
+            _check(dt == _E4M3 or (not fp8_only and dt in _HALF_DTYPES),
+                   "k_cache must be float8_e4m3fn" + ("" if fp8_only else ", bfloat16 or float16"))
+            _check(v_cache.dtype == dt, "v_cache must have k_cache's dtype")
+            _check(k_cache.dim() == 4, "k_cache must be [pages,page_size,Hkv,D]")
+            _check(v_cache.get_device() == dev, "v_cache: tensors must be on the same device")
+        shape = k_cache.shape
+        _check(v_cache.shape == shape, "v_cache must match k_cache")
+        pages, page, hkv, d = shape
+        k0, k1, k2, k3 = k_cache.stride()
+        v0, v1, v2, v3 = v_cache.stride()
+        _check(k3 == 1 and v3 == 1, "k_cache and v_cache must have contiguous last dimension")
+        scales = 0
         if kv_scales is not None:
-            _check(kv_scales.is_cuda and kv_scales.device == k_cache.device,
-                   "kv_scales: tensors must be on the same device")
-            _check(dt == torch.float8_e4m3fn, "kv_scales belong to a float8_e4m3fn cache")
-            _check(kv_scales.dtype in _SCALE_DTYPES, "kv_scales must be uint8 or float8_e8m0fnu")
-            _check(kv_scales.shape == (pages, hkv, page, 2) and kv_scales.is_contiguous(),
-                   "kv_scales must be a contiguous [pages,Hkv,page_size,2] tensor")
-        n = k_cache.element_size()
-        return MacPagedCache(_CACHE_SIZE, ABI_VERSION, k_cache.data_ptr(), v_cache.data_ptr(),
-                             None if kv_scales is None else kv_scales.data_ptr(), pages,
-                             ks[0] * n, ks[1] * n, ks[2] * n, vs[0] * n, vs[1] * n, vs[2] * n, page, hkv, d,
-                             _DTYPE_CODES[dt], float(k_scale), float(v_scale))
+            if not (kv_scales.get_device() == dev and dt == _E4M3 and kv_scales.dtype in _SCALE_DTYPES
+                    and kv_scales.shape == (pages, hkv, page, 2) and kv_scales.is_contiguous()):
+                _check(kv_scales.get_device() == dev, "kv_scales: tensors must be on the same device")
+                _check(dt == _E4M3, "kv_scales belong to a float8_e4m3fn cache")
+                _check(kv_scales.dtype in _SCALE_DTYPES, "kv_scales must be uint8 or float8_e8m0fnu")
+                raise RuntimeError("kv_scales must be a contiguous [pages,Hkv,page_size,2] tensor")
+            scales = kv_scales.data_ptr()
+        if dt != _E4M3:
+            k0, k1, k2, v0, v1, v2 = 2 * k0, 2 * k1, 2 * k2, 2 * v0, 2 * v1, 2 * v2
+        block = _pack_cache(_CACHE_SIZE, ABI_VERSION, k_cache.data_ptr(), v_cache.data_ptr(), scales, pages, k0, k1,
+                            k2, v0, v1, v2, page, hkv, d, _DTYPE_CODES[dt], k_scale, v_scale)
+        return block, dev, hkv, d
+
+    def _call(self, fn, dev: int, *args) -> None:
+        """fn(*args, stream) on the tensors' device and its current stream."""
+        if torch._C._cuda_getDevice() == dev:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        if rc != 0:
+            _raise_on(self._lib, rc)
 
     def mac_paged_cache_write_fp8(self, k, v, k_cache, v_cache, kv_scales, cache_locs, k_scale: float = 1.0,
                                   v_scale: float = 1.0) -> None:
@@ -1089,18 +1146,15 @@ class PagedCacheExtension:
         strides) into the slots cache_locs (int32 or int64: page * page_size +
         slot; locs outside the cache are skipped, negative ones pad; a slot may
         be named once per call)."""
-        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
-        dev = k_cache.device
-        _check_rows(k, "k", dev, c.Hkv, c.D)
-        _check_rows(v, "v", dev, c.Hkv, c.D)
-        _check(v.dtype == k.dtype and v.shape == k.shape, "v must match k")
-        n = k.shape[0]
-        _check_vector(cache_locs, "cache_locs", dev, (torch.int32, torch.int64), n)
-        with _on_device(dev):
-            rc = self._lib.mac_paged_cache_write_fp8(
-                ctypes.byref(c), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                _DTYPE_CODES[k.dtype], cache_locs.data_ptr(), cache_locs.dtype == torch.int64, n, _stream(dev))
-        _raise_on(self._lib, rc)
+        c, dev, hkv, d = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        shape, ks = _check_rows(k, "k", dev, hkv, d)
+        v_shape, vs = _check_rows(v, "v", dev, hkv, d)
+        dt = k.dtype
+        _check(v.dtype == dt and v_shape == shape, "v must match k")
+        n = shape[0]
+        _check_vector(cache_locs, "cache_locs", dev, _INDEX_DTYPES, n)
+        self._call(self._lib.mac_paged_cache_write_fp8, dev, c, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                   _DTYPE_CODES[dt], cache_locs.data_ptr(), cache_locs.dtype == torch.int64, n)
 
     def mac_paged_rope_write_fp8(self, q, k, v, k_cache, v_cache, kv_scales, cos_sin_cache, positions, cache_locs,
                                  is_neox: bool = True, k_scale: float = 1.0, v_scale: float = 1.0, q_out=None):
@@ -1109,60 +1163,55 @@ class PagedCacheExtension:
         cache_locs.  q [tokens, Hq, D], k, v [tokens, Hkv, D]; cos_sin_cache
         float32 [positions, rotary_dim]; positions int32 or int64 (clamped into
         the table)."""
-        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
-        dev = k_cache.device
-        _check_rows(q, "q", dev, None, c.D)
-        _check_rows(k, "k", dev, c.Hkv, c.D)
-        _check_rows(v, "v", dev, c.Hkv, c.D)
-        _check(q.dtype == k.dtype and v.dtype == k.dtype, "q, k and v must have the same dtype")
-        n, hq = q.shape[0], q.shape[1]
-        _check(k.shape[0] == n and v.shape[0] == n, "q/k/v batch mismatch")
-        _check(cos_sin_cache.is_cuda and cos_sin_cache.device == dev,
-               "cos_sin_cache: tensors must be on the same device")
-        _check(cos_sin_cache.dtype == torch.float32, "cos_sin_cache has wrong dtype")
-        _check(cos_sin_cache.dim() == 2, "cos_sin_cache must have rank 2")
-        _check(cos_sin_cache.stride(1) == 1, "cos_sin_cache must have contiguous last dimension")
-        rot = cos_sin_cache.shape[1]
-        _check(0 < rot <= c.D and rot % 2 == 0, "invalid rotary_dim")
-        ints = (torch.int32, torch.int64)
-        _check_vector(positions, "positions", dev, ints, n)
-        _check_vector(cache_locs, "cache_locs", dev, ints, n)
+        c, dev, hkv, d = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        shape, qs = _check_rows(q, "q", dev, None, d)
+        k_shape, ks = _check_rows(k, "k", dev, hkv, d)
+        v_shape, vs = _check_rows(v, "v", dev, hkv, d)
+        dt = q.dtype
+        _check(k.dtype == dt and v.dtype == dt, "q, k and v must have the same dtype")
+        n, hq = shape[0], shape[1]
+        _check(k_shape[0] == n and v_shape[0] == n, "q/k/v batch mismatch")
+        if not (cos_sin_cache.get_device() == dev and cos_sin_cache.dtype == torch.float32 and cos_sin_cache.dim() == 2):
+            _check(cos_sin_cache.get_device() == dev, "cos_sin_cache: tensors must be on the same device")
+            _check(cos_sin_cache.dtype == torch.float32, "cos_sin_cache has wrong dtype")
+            raise RuntimeError("cos_sin_cache must have rank 2")
+        rows, rot = cos_sin_cache.shape
+        cs0, cs1 = cos_sin_cache.stride()
+        _check(cs1 == 1, "cos_sin_cache must have contiguous last dimension")
+        _check(0 < rot <= d and rot % 2 == 0, "invalid rotary_dim")
+        _check_vector(positions, "positions", dev, _INDEX_DTYPES, n)
+        _check_vector(cache_locs, "cache_locs", dev, _INDEX_DTYPES, n)
         if q_out is None:
-            q_out = torch.empty((n, hq, c.D), device=dev, dtype=q.dtype)
-        _check(q_out.shape == q.shape and q_out.dtype == q.dtype and q_out.device == dev and q_out.is_contiguous(),
-               "q_out must be a contiguous tensor shaped like q")
-        a = MacPagedRopeArgs(_PAGED_ROPE_SIZE, ABI_VERSION, q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0),
-                             q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), q_out.data_ptr(),
-                             cos_sin_cache.data_ptr(), cos_sin_cache.shape[0], cos_sin_cache.stride(0),
-                             positions.data_ptr(), cache_locs.data_ptr(), n, hq, rot, bool(is_neox),
-                             _DTYPE_CODES[q.dtype], positions.dtype == torch.int64, cache_locs.dtype == torch.int64)
-        with _on_device(dev):
-            rc = self._lib.mac_paged_rope_write_fp8(ctypes.byref(c), ctypes.byref(a), _stream(dev))
-        _raise_on(self._lib, rc)
+            q_out = torch.empty(shape, device=q.device, dtype=dt)
+        else:
+            _check_result(q_out, shape, dt, dev, "q_out must be a contiguous tensor shaped like q")
+        a = _pack_rope(_PAGED_ROPE_SIZE, ABI_VERSION, q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1],
+                       vs[0], vs[1], q_out.data_ptr(), cos_sin_cache.data_ptr(), rows, cs0, positions.data_ptr(),
+                       cache_locs.data_ptr(), n, hq, rot, bool(is_neox), _DTYPE_CODES[dt],
+                       positions.dtype == torch.int64, cache_locs.dtype == torch.int64)
+        self._call(self._lib.mac_paged_rope_write_fp8, dev, c, a)
         return q_out
 
     def mac_paged_cache_read_fp8(self, k_cache, v_cache, kv_scales, kv_indices, dtype: torch.dtype = torch.bfloat16,
                                  k_scale: float = 1.0, v_scale: float = 1.0, out_k=None, out_v=None):
         """K and V [rows, Hkv, D] of the slots kv_indices (int32 or int64) in
         dtype (bf16, fp16 or fp32); slots outside the cache read as zeros."""
-        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
-        dev = k_cache.device
-        _check(dtype in (torch.float32, torch.bfloat16, torch.float16), "dtype must be float32, bfloat16 or float16")
-        _check_vector(kv_indices, "kv_indices", dev, (torch.int32, torch.int64))
-        shape = (kv_indices.shape[0], c.Hkv, c.D)
-        outs = []
-        for name, t in (("out_k", out_k), ("out_v", out_v)):
-            if t is None:
-                t = torch.empty(shape, device=dev, dtype=dtype)
-            _check(t.shape == shape and t.dtype == dtype and t.device == dev and t.is_contiguous(),
-                   f"{name} must be a contiguous [rows,Hkv,D] tensor of dtype")
-            outs.append(t)
-        with _on_device(dev):
-            rc = self._lib.mac_paged_cache_read_fp8(
-                ctypes.byref(c), kv_indices.data_ptr(), kv_indices.dtype == torch.int64, shape[0], outs[0].data_ptr(),
-                outs[1].data_ptr(), _DTYPE_CODES[dtype], _stream(dev))
-        _raise_on(self._lib, rc)
-        return outs[0], outs[1]
+        c, dev, hkv, d = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale)
+        _check(dtype in _HALF_DTYPES or dtype == torch.float32, "dtype must be float32, bfloat16 or float16")
+        _check_vector(kv_indices, "kv_indices", dev, _INDEX_DTYPES)
+        n = kv_indices.size(0)
+        shape = (n, hkv, d)
+        if out_k is None:
+            out_k = torch.empty(shape, device=k_cache.device, dtype=dtype)
+        else:
+            _check_result(out_k, shape, dtype, dev, "out_k must be a contiguous [rows,Hkv,D] tensor of dtype")
+        if out_v is None:
+            out_v = torch.empty(shape, device=k_cache.device, dtype=dtype)
+        else:
+            _check_result(out_v, shape, dtype, dev, "out_v must be a contiguous [rows,Hkv,D] tensor of dtype")
+        self._call(self._lib.mac_paged_cache_read_fp8, dev, c, kv_indices.data_ptr(), kv_indices.dtype == torch.int64, n,
+                   out_k.data_ptr(), out_v.data_ptr(), _DTYPE_CODES[dtype])
+        return out_k, out_v
 
     def mac_paged_chunk_attention(self, q, k_cache, v_cache, qo_indptr, kv_lens, page_table, sm_scale: float,
                                   kv_scales=None, k_scale: float = 1.0, v_scale: float = 1.0, window_left: int = -1,
@@ -1173,53 +1222,60 @@ class PagedCacheExtension:
         page_table (int32 [rows, pages], row req_ids[b] or b).  Returns out
         (q's dtype) and the natural-log lse (float32 [total_q, Hq]); rows that
         see no key get 0 and -inf, rows of no request are left as they are."""
-        c = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only=False)
-        dev = k_cache.device
-        _check_rows(q, "q", dev, None, c.D)
-        _check(k_cache.dtype == torch.float8_e4m3fn or k_cache.dtype == q.dtype,
-               "k_cache must be float8_e4m3fn or of q's dtype")
-        total_q, hq = q.shape[0], q.shape[1]
-        _check(hq % c.Hkv == 0 if c.Hkv else False, "Hq must be a multiple of Hkv")
-        i32 = (torch.int32,)
-        _check_vector(qo_indptr, "qo_indptr", dev, i32)
-        batch = qo_indptr.shape[0] - 1
+        c, dev, hkv, d = self._cache(k_cache, v_cache, kv_scales, k_scale, v_scale, fp8_only=False)
+        shape, qs = _check_rows(q, "q", dev, None, d)
+        dt = q.dtype
+        _check(kv_scales is not None or k_cache.dtype in (_E4M3, dt), "k_cache must be float8_e4m3fn or of q's dtype")
+        total_q, hq = shape[0], shape[1]
+        _check(hkv > 0 and hq % hkv == 0, "Hq must be a multiple of Hkv")
+        _check_vector(qo_indptr, "qo_indptr", dev, _I32_ONLY)
+        batch = qo_indptr.size(0) - 1
         _check(batch >= 0, "qo_indptr must be [B+1]")
-        _check_vector(kv_lens, "kv_lens", dev, i32, batch)
+        _check_vector(kv_lens, "kv_lens", dev, _I32_ONLY, batch)
+        ids = 0
         if req_ids is not None:
-            _check_vector(req_ids, "req_ids", dev, i32, batch)
-        _check(page_table.is_cuda and page_table.device == dev, "page_table: tensors must be on the same device")
-        _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 [rows,pages]")
+            _check_vector(req_ids, "req_ids", dev, _I32_ONLY, batch)
+            ids = req_ids.data_ptr()
+        if not (page_table.get_device() == dev and page_table.dtype == torch.int32 and page_table.dim() == 2):
+            _check(page_table.get_device() == dev, "page_table: tensors must be on the same device")
+            raise RuntimeError("page_table must be int32 [rows,pages]")
         rows, cols = page_table.shape
-        _check(cols <= 1 or page_table.stride(1) == 1, "page_table must have contiguous rows")
+        ts0, ts1 = page_table.stride()
+        _check(cols <= 1 or ts1 == 1, "page_table must have contiguous rows")
         _check(req_ids is not None or rows >= batch, "page_table has fewer rows than the batch")
-        if q.data_ptr() % 16 or q.stride(0) % 8 or q.stride(1) % 8:
-            q = q.contiguous()  # rows that 16-byte loads cannot read
-            if q.data_ptr() % 16:
-                q = q.clone()
+        q_ptr = q.data_ptr()
+        if q_ptr % 16 or qs[0] % 8 or qs[1] % 8:  # rows that 16-byte loads cannot read
+            q = q.clone(memory_format=torch.contiguous_format)
+            q_ptr, qs = q.data_ptr(), q.stride()
         if out is None:
-            out = torch.empty((total_q, hq, c.D), device=dev, dtype=q.dtype)
+            out = torch.empty(shape, device=q.device, dtype=dt)
+        else:
+            _check_result(out, shape, dt, dev, "out must be a contiguous tensor shaped like q")
         if out_lse is None:
-            out_lse = torch.empty((total_q, hq), device=dev, dtype=torch.float32)
-        _check(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.is_contiguous(),
-               "out must be a contiguous tensor shaped like q")
-        _check(out_lse.shape == (total_q, hq) and out_lse.dtype == torch.float32 and out_lse.device == dev
-               and out_lse.is_contiguous(), "out_lse must be contiguous f32 [total_q,Hq]")
-        a = MacPagedAttentionArgs(_PAGED_ATTENTION_SIZE, ABI_VERSION, q.data_ptr(), q.stride(0), q.stride(1),
-                                  qo_indptr.data_ptr(), kv_lens.data_ptr(), page_table.data_ptr(),
-                                  page_table.stride(0), None if req_ids is None else req_ids.data_ptr(),
-                                  out.data_ptr(), out_lse.data_ptr(), total_q, batch, hq, rows, cols,
-                                  _DTYPE_CODES[q.dtype], int(window_left), float(sm_scale), float(logit_cap))
-        lib = self._lib
-        with _on_device(dev):
-            # the partial states of keys that several workgroups share, from
-            # PyTorch's allocator (its stream-ordered reuse and graph pools keep
-            # it safe across streams and captures)
-            n = lib.mac_paged_chunk_attention_workspace(ctypes.byref(c), ctypes.byref(a))
-            ws = torch.empty(n, device=dev, dtype=torch.uint8) if n > 0 else None
-            rc = lib.mac_paged_chunk_attention(ctypes.byref(c), ctypes.byref(a), None if ws is None else ws.data_ptr(),
-                                               max(n, 0), _stream(dev))
-        _raise_on(lib, rc)
+            out_lse = torch.empty((total_q, hq), device=q.device, dtype=torch.float32)
+        else:
+            _check_result(out_lse, (total_q, hq), torch.float32, dev, "out_lse must be contiguous f32 [total_q,Hq]")
+        a = _pack_attention(_PAGED_ATTENTION_SIZE, ABI_VERSION, q_ptr, qs[0], qs[1], qo_indptr.data_ptr(),
+                            kv_lens.data_ptr(), page_table.data_ptr(), ts0, ids, out.data_ptr(), out_lse.data_ptr(),
+                            total_q, batch, hq, rows, cols, _DTYPE_CODES[dt], min(int(window_left), _ANY_WINDOW), sm_scale, logit_cap)
+        if torch._C._cuda_getDevice() == dev:
+            self._attend(c, a, q.device, dev)
+        else:
+            with torch.cuda.device(dev):
+                self._attend(c, a, q.device, dev)
         return out, out_lse
+
+    def _attend(self, c: bytes, a: bytes, device: torch.device, index: int) -> None:
+        """The launch, with room for the partial states of keys that several
+        workgroups share from PyTorch's allocator (its stream-ordered reuse and
+        graph pools keep it safe across streams and captures)."""
+        lib = self._lib
+        n = lib.mac_paged_chunk_attention_workspace(c, a)
+        ws = torch.empty(n, device=device, dtype=torch.uint8) if n > 0 else None
+        rc = lib.mac_paged_chunk_attention(c, a, None if ws is None else ws.data_ptr(), max(n, 0),
+                                           torch._C._cuda_getCurrentRawStream(index))
+        if rc != 0:
+            _raise_on(lib, rc)
 
 
 @lru_cache(maxsize=1)

@@ -431,6 +431,16 @@ def test_against_the_window_kernel(ext):
     assert torch.all((out.double() - o.double()).abs() <= 2 * to) and torch.all((lse - l).double().abs() <= 2 * tl)
 
 
+def test_a_window_wider_than_any_request(ext):
+    p = Problem([5, 40], [300, 77], 8, 2, 128, 16)
+    want = p.run(ext)
+    for w in (299, 1 << 30, (1 << 31) - 1, 1 << 40):
+        got = p.run(ext, window_left=w)
+        if w >= 1 << 30:
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        p.check(got)
+
+
 def test_empty_batches(ext):
     p = Problem([1], [9], 2, 1, 64, 16)
     none = torch.empty(0, 2, 64, device=DEV, dtype=BF)
@@ -473,4 +483,6 @@ def test_refusals(ext):
     refused("positive", kv_scales=None, v_scale=-1.0)
     refused("out must be", out=torch.empty(3, 8, 64, device=DEV, dtype=BF))
     refused("out_lse must be", out_lse=torch.empty(3, 8, device=DEV, dtype=BF))
+    refused("same strides", k_cache=p.kc, v_cache=p.vc.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(ph.F8))
+    refused("out of range", kv_scales=None, k_scale=1e300)
     refused("power of two", k_cache=p.kc[:, :12], v_cache=p.vc[:, :12], kv_scales=None)
