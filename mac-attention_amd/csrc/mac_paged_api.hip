@@ -72,7 +72,13 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int64_t worst = static_cast<int64_t>(B) * ((total_q * G + ch.cols - 1) / ch.cols) * c.Hkv;
   if (worst >= INT_MAX) return false;
   const int resident = variant(q_dtype, c.cache_dtype).resident(c.D, ch.body, B);
-  ch.stream = ch.body <= kBodyStream32 || tasks < 2 * static_cast<int64_t>(resident);
+  // The tile body streams its keys where its tasks alone leave a quarter of the GPU
+  // idle; else workgroups that take whole tasks, in step over the same keys, share
+  // them in L2 and write no partial states.  Streamed / whole, 4 heads per group (us):
+  // 512 rows over 32K keys (128 tasks of 512 resident) 377 / 893, over 8K 149 / 240,
+  // 1024 over 8K (256) 260 / 248, 2048 over 2K (512) 208 / 83, over 8K 444 / 320; 24
+  // ragged requests, 64 dims, 592 bounding tasks of 768, 158 / 144.
+  ch.stream = ch.body <= kBodyStream32 || 4 * tasks < 3 * static_cast<int64_t>(resident);
   ch.grid = resident;
   if (!ch.stream) {
     ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));

@@ -484,5 +484,6 @@ def test_refusals(ext):
     refused("out must be", out=torch.empty(3, 8, 64, device=DEV, dtype=BF))
     refused("out_lse must be", out_lse=torch.empty(3, 8, device=DEV, dtype=BF))
     refused("same strides", k_cache=p.kc, v_cache=p.vc.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(ph.F8))
-    refused("out of range", kv_scales=None, k_scale=1e300)
+    refused("positive", kv_scales=None, k_scale=1e300)
+    refused("out of range", window_left=-(1 << 40))
     refused("power of two", k_cache=p.kc[:, :12], v_cache=p.vc[:, :12], kv_scales=None)
