@@ -51,7 +51,11 @@ size_t up16(size_t n) { return (n + 15) / 16 * 16; }
 bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B, int64_t max_keys, Choice& ch) {
   const int G = Hq / c.Hkv;
   const int64_t cols = (total_q + B - 1) / B * G;  // columns of a request of average length
-  ch.body = cols <= 16 ? kBodyStream16 : (cols <= 32 ? kBodyStream32 : (cols <= 64 ? kBodyTile64 : kBodyTile128));
+  // 17 to 32 columns: the stream body where a wave's registers hold them (32 requests
+  // of 4 rows of 8 heads, stream / tile, us: 8-bit rows of 128 dims over 16K keys 129 /
+  // 147, of 64 over 26K 123 / 131, 16-bit of 64 175 / 186; 16-bit of 128 dims 272 / 237)
+  const bool stream32 = cols <= 32 && (c.cache_dtype == MAC_DTYPE_E4M3 || c.D == 64);
+  ch.body = cols <= 16 ? kBodyStream16 : (stream32 ? kBodyStream32 : (cols <= 64 ? kBodyTile64 : kBodyTile128));
   if (c.D > 128) ch.body = kBodyTile64;  // (the only one whose states and operands of 256 dims fit a wave's registers)
   const int room = kBodyCols[ch.body];
   ch.cols = G <= room ? room / G * G : room;  // whole rows where a row's heads fit

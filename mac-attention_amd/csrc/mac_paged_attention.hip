@@ -1036,7 +1036,9 @@ Kernel body_kernel(int body) {
   if constexpr (D <= 128) {
     switch (body) {
       case kBodyStream16: return stream_kernel<D, 1>;
-      case kBodyStream32: return stream_kernel<D, 2>;
+      case kBodyStream32:
+        if constexpr (kF8 || D == 64) return stream_kernel<D, 2>;
+        return nullptr;
       case kBodyTile64: return tile_kernel<D, 1, 64, 2>;
       default: return tile_kernel<D, 2, 64, (D == 64 ? 3 : 2)>;
     }
