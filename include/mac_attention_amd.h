@@ -472,11 +472,16 @@ MAC_API int mac_paged_cache_read_fp8(const MacPagedCache* cache, const void* kv_
  * rows.
  *   q       [total_q, Hq, D] of q_dtype (MAC_DTYPE_BF16 / F16), token and head
  *           strides in elements, rows 16-byte aligned
- *   cache   of q_dtype or MAC_DTYPE_E4M3; D 64, 128 or 256; any group size
+ *   cache   of q_dtype or MAC_DTYPE_E4M3 (values beyond fp16's range are infinite
+ *           for fp16 queries); D 64, 128 or 256; any group size; the same strides,
+ *           below 2^32 bytes, for K and V
  *   out     [total_q, Hq, D] of q_dtype, out_lse f32 [total_q, Hq], contiguous
  *   page_table i32 [table_rows, table_cols], rows table_stride entries apart
+ * Infinities and NaN in a key that a row sees reach that row (with the others'
+ * weights, as in a softmax over them); in keys that it does not see they do not.
  * Sums are fp32; weights are rounded to q_dtype for their product with V.  A
- * call's results depend on its inputs and shapes only.
+ * call's results depend on its inputs, shapes and the device only.  At most 4096
+ * requests.
  */
 typedef struct MacPagedAttentionArgs {
   uint32_t struct_size; /* sizeof(MacPagedAttentionArgs) */

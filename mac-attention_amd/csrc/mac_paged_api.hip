@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -206,6 +207,11 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   p.q_scale = static_cast<float>(a->logit_cap > 0 ? 1.0 : raw * log2e);
   p.cap_in = a->logit_cap > 0 ? static_cast<float>(2.0 * log2e * raw / a->logit_cap) : 0.0f;
   p.cap_out = static_cast<float>(a->logit_cap * log2e);
+  // (scores are scaled in fp32: a factor that is 0 or infinite there would turn
+  // masked scores into NaN)
+  REQUIRE(p.q_scale >= FLT_MIN && std::isfinite(p.q_scale), "sm_scale * k_scale does not fit fp32");
+  REQUIRE(a->logit_cap == 0 || (p.cap_in >= FLT_MIN && std::isfinite(p.cap_in) && p.cap_out >= FLT_MIN && std::isfinite(p.cap_out)),
+          "logit_cap does not fit fp32 with sm_scale");
   p.v_scale = c->v_scale;
   const hipError_t e = variant(a->q_dtype, c->cache_dtype).launch(p, c->D, ch.body, ch.grid, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return mac::fail(MAC_ERR_HIP, "paged chunk attention: %s", hipGetErrorString(e));

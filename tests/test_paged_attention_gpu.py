@@ -431,6 +431,43 @@ def test_against_the_window_kernel(ext):
     assert torch.all((out.double() - o.double()).abs() <= 2 * to) and torch.all((lse - l).double().abs() <= 2 * tl)
 
 
+@pytest.mark.parametrize("rows", [1, 6, 90])
+def test_a_query_that_is_not_finite_spares_the_others(ext, rows):
+    p = Problem([rows, rows], [rows + 200, rows + 30], 8, 2, 128, 16)
+    want = p.run(ext)
+    p.q[rows // 2, 3, 5] = math.nan
+    p.q[rows + rows // 3, 1] = math.inf
+    out, lse = p.run(ext)
+    hit = torch.zeros(2 * rows, 8, dtype=torch.bool, device=DEV)
+    hit[rows // 2, 3] = hit[rows + rows // 3, 1] = True
+    assert torch.isnan(out[hit]).all() and torch.isnan(lse[hit]).all()
+    assert torch.equal(out[~hit], want[0][~hit]) and torch.equal(lse[~hit], want[1][~hit])
+
+
+@pytest.mark.parametrize("rows,hq", [(1, 4), (20, 16)])
+def test_the_most_requests(ext, rows, hq):
+    """4096 requests (decode, and tasks of 128 columns), checked on a sample."""
+    new = [rows] * 4096
+    lens = [rows + 7 * i % 50 for i in range(4096)]
+    p = Problem(new, lens, hq, 2, 64, 4, seed=8)
+    out, lse = p.run(ext)
+    for b in (0, 1, 77, 2048, 4094, 4095):
+        at = b * rows
+        want = ph.attention(p.q[at:at + rows], p.k, p.v, [rows], [lens[b]], p.table[b:b + 1], 4, p.kc.shape[0], p.sm)
+        ph.assert_close(out[at:at + rows], want[0], want[2], f"out of request {b}")
+        ph.assert_close(lse[at:at + rows], want[1], want[3], f"lse of request {b}")
+    with pytest.raises(RuntimeError, match="4096"):
+        qo, kl = _i32([0] * 4098), _i32([1] * 4097)
+        ext.mac_paged_chunk_attention(p.q, p.kc, p.vc, qo, kl, p.table[:1].expand(4097, -1), p.sm, kv_scales=p.sc)
+
+
+def test_windows_past_the_table(ext):
+    """Rows whose whole window lies past the keys that the table names."""
+    p = Problem([2, 40, 1], [500, 300, 900], 4, 2, 64, 16, window=30)
+    p.table = p.table[:, :10].contiguous()
+    p.check(p.run(ext))
+
+
 def test_a_window_wider_than_any_request(ext):
     p = Problem([5, 40], [300, 77], 8, 2, 128, 16)
     want = p.run(ext)
@@ -479,6 +516,8 @@ def test_refusals(ext):
     refused("sm_scale", sm_scale=0.0)
     refused("sm_scale", sm_scale=float("inf"))
     refused("logit_cap", logit_cap=-1.0)
+    refused("does not fit fp32", sm_scale=1e-60)
+    refused("does not fit fp32", logit_cap=1e300)
     refused("takes no k_scale", k_scale=0.5)
     refused("positive", kv_scales=None, v_scale=-1.0)
     refused("out must be", out=torch.empty(3, 8, 64, device=DEV, dtype=BF))
