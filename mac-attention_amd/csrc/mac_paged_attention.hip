@@ -939,48 +939,59 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
 // ---------------------------------------------------------------- combine ---
 
 // Stream form, second launch: the partial states of a task that several
-// workgroups shared.  One workgroup per (row, query head); the waves take every
-// fourth piece, four loads ahead.  Rows of whole tasks return at once.
-template <int D>
-__global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
-  PagedArgs& p = fresh_args();
-  constexpr int kV = D / 64;  // floats per lane
-  __shared__ int s_b;
-  __shared__ float s_o[4][D], s_m[4], s_l[4];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int64_t row = blockIdx.x / p.Hq;
-  const int head = static_cast<int>(blockIdx.x - row * p.Hq);
-  if (tid == 0) s_b = -1;
-  __syncthreads();
-  for (int b = tid; b < p.B; b += 256)
-    if (p.qo_indptr[b] <= row && row < p.qo_indptr[b + 1]) s_b = b;
-  __syncthreads();
-  const int b = __builtin_amdgcn_readfirstlane(s_b);
-  if (b < 0) return;  // a row of no request
-  const PagedRequest r = paged_request(p, b);
-  if (r.n == 0) return;
-  const int total = p.plan[p.B], groups = stream_groups(p, total);
+// workgroups shared.  Rows of whole tasks return at once.
+//
+// Where the pieces of query row `row` and head `head` of request b lie: the
+// workgroups first .. first + n - 1, n = 0 for a task that one workgroup had.
+struct Pieces {
+  int first, n;
+  bool at_start;  // the first one's run begins with the task
+  int64_t offset;  // of the column in a slot
+  __device__ __forceinline__ int64_t place(int i, int64_t slot_columns) const {
+    const int64_t slot = 2 * static_cast<int64_t>(first + i) + (i == 0 && !at_start ? 1 : 0);
+    return slot * slot_columns + offset;
+  }
+};
+__device__ __forceinline__ Pieces find_pieces(PagedArgs& p, const PagedRequest& r, int before, int total, int row, int head, int kc) {
+  const int groups = stream_groups(p, total);
   const int hkv = head / p.G;
-  const int gc = static_cast<int>(row - r.q0) * p.G + head - hkv * p.G;
+  const int gc = (row - r.q0) * p.G + head - hkv * p.G;
   const int ct = gc / p.cols, col = gc - ct * p.cols;
   const int group = hkv >> p.heads_shift;
-  const int first = p.plan[b] + (group * r.tasks + ct) * r.units;
-  const int wa = stream_owner(first, total, groups), wb = stream_owner(first + r.units - 1, total, groups);
-  if (wa == wb) return;  // stored by its workgroup
-  const bool at_start = stream_begin(wa, total, groups) == first;
-  const int n = wb - wa + 1;
-  auto place = [&](int i) {
-    const int64_t slot = 2 * static_cast<int64_t>(wa + i) + (i == 0 && !at_start ? 1 : 0);
-    return ((slot << p.heads_shift) + hkv - (group << p.heads_shift)) * kc + col;
-  };
-  float m = -INFINITY, l = 0.0f, o[kV] = {};
-  constexpr int kB = 4;
-  for (int i0 = wave; i0 < n; i0 += 4 * kB) {
+  const int unit = before + (group * r.tasks + ct) * r.units;
+  Pieces x;
+  x.first = stream_owner(unit, total, groups);
+  x.n = stream_owner(unit + r.units - 1, total, groups) - x.first;
+  x.n = x.n > 0 ? x.n + 1 : 0;
+  x.at_start = stream_begin(x.first, total, groups) == unit;
+  x.offset = static_cast<int64_t>(hkv - (group << p.heads_shift)) * kc + col;
+  return x;
+}
+// The request that a row belongs to (-1: none), for a whole workgroup.
+__device__ __forceinline__ int request_of_row(PagedArgs& p, int row) {
+  __shared__ int s_b;
+  if (threadIdx.x == 0) s_b = -1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < p.B; b += 256)
+    if (p.qo_indptr[b] <= row && row < p.qo_indptr[b + 1]) s_b = b;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(s_b);
+}
+// A wave's state over the pieces i0, i0 + step, ..: lane l holds dims l + 64 j.
+template <int kV>
+struct Joined {
+  float m, l, o[kV];
+};
+template <int kV>
+__device__ __forceinline__ Joined<kV> join_pieces(PagedArgs& p, const Pieces& x, int64_t slot_columns, int i0, int step) {
+  constexpr int D = 64 * kV, kB = 4;  // pieces' loads in flight
+  const int lane = threadIdx.x & 63;
+  Joined<kV> s = {-INFINITY, 0.0f, {}};
+  for (; i0 < x.n; i0 += step * kB) {
     float pm[kB], pl[kB], po[kB][kV];
 #pragma unroll
     for (int u = 0; u < kB; ++u) {
-      const int64_t at = place(min(i0 + 4 * u, n - 1));
+      const int64_t at = x.place(min(i0 + step * u, x.n - 1), slot_columns);
       pm[u] = p.part_ml[2 * at];
       pl[u] = p.part_ml[2 * at + 1];
 #pragma unroll
@@ -988,20 +999,40 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
     }
 #pragma unroll
     for (int u = 0; u < kB; ++u) {
-      if (i0 + 4 * u >= n) break;
-      const float mn = max3_nonan(m, pm[u], pm[u]);
-      const float fa = m == mn ? 1.0f : fast_exp2(m - mn), fb = pm[u] == mn ? 1.0f : fast_exp2(pm[u] - mn);
-      m = mn;
-      l = l * fa + pl[u] * fb;
+      if (i0 + step * u >= x.n) break;
+      const float mn = max3_nonan(s.m, pm[u], pm[u]);
+      const float fa = s.m == mn ? 1.0f : fast_exp2(s.m - mn), fb = pm[u] == mn ? 1.0f : fast_exp2(pm[u] - mn);
+      s.m = mn;
+      s.l = s.l * fa + pl[u] * fb;
 #pragma unroll
-      for (int j = 0; j < kV; ++j) o[j] = o[j] * fa + po[u][j] * fb;
+      for (int j = 0; j < kV; ++j) s.o[j] = s.o[j] * fa + po[u][j] * fb;
     }
   }
+  return s;
+}
+
+// Few rows, each in many pieces (stream body): one workgroup per (row, query
+// head), its waves take every fourth piece.
+template <int D>
+__global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
+  PagedArgs& p = fresh_args();
+  constexpr int kV = D / 64;
+  __shared__ float s_o[4][D], s_m[4], s_l[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x / p.Hq, head = blockIdx.x - row * p.Hq;
+  const int b = request_of_row(p, row);
+  if (b < 0) return;
+  const PagedRequest r = paged_request(p, b);
+  if (r.n == 0) return;
+  const Pieces x = find_pieces(p, r, p.plan[b], p.plan[p.B], row, head, kc);
+  if (x.n == 0) return;  // stored by its workgroup
+  const Joined<kV> s = join_pieces<kV>(p, x, static_cast<int64_t>(kc) << p.heads_shift, wave, 4);
 #pragma unroll
-  for (int j = 0; j < kV; ++j) s_o[wave][64 * j + lane] = o[j];
+  for (int j = 0; j < kV; ++j) s_o[wave][64 * j + lane] = s.o[j];
   if (lane == 0) {
-    s_m[wave] = m;
-    s_l[wave] = l;
+    s_m[wave] = s.m;
+    s_l[wave] = s.l;
   }
   __syncthreads();
   float mx = s_m[0], lt = 0.0f;
@@ -1013,7 +1044,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
     f[w] = s_m[w] == mx ? 1.0f : fast_exp2(s_m[w] - mx);
     lt += s_l[w] * f[w];
   }
-  const int64_t at = row * p.Hq + head;
+  const int64_t at = static_cast<int64_t>(row) * p.Hq + head;
   const float inv = lt == 0.0f ? 0.0f : p.v_scale / lt;
   for (int d = 2 * tid; d < D; d += 512) {
     float y[2] = {0.0f, 0.0f};
@@ -1027,9 +1058,36 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   if (tid == 0) p.lse[at] = lt == 0.0f ? -INFINITY : (mx + fast_log2(lt)) * kLn2;
 }
 
+// Many rows in few pieces (tile body): one workgroup per row, a wave per query
+// head in turn.
+template <int D>
+__global__ void __launch_bounds__(256) combine_rows_kernel(PagedParams, int kc) {
+  PagedArgs& p = fresh_args();
+  constexpr int kV = D / 64;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = blockIdx.x;
+  const int b = request_of_row(p, row);
+  if (b < 0) return;
+  const PagedRequest r = paged_request(p, b);
+  if (r.n == 0) return;
+  const int before = p.plan[b], total = p.plan[p.B];
+  for (int head = wave; head < p.Hq; head += 4) {
+    const Pieces x = find_pieces(p, r, before, total, row, head, kc);
+    if (x.n == 0) continue;
+    const Joined<kV> s = join_pieces<kV>(p, x, static_cast<int64_t>(kc) << p.heads_shift, 0, 1);
+    const int64_t at = static_cast<int64_t>(row) * p.Hq + head;
+    const float inv = s.l == 0.0f ? 0.0f : p.v_scale / s.l;
+#pragma unroll
+    for (int j = 0; j < kV; ++j) p.out[at * D + 64 * j + lane] = static_cast<uint16_t>(E::pack2(s.o[j] * inv, 0.0f));
+    if (lane == 0) p.lse[at] = s.l == 0.0f ? -INFINITY : (s.m + fast_log2(s.l)) * kLn2;
+  }
+}
+
 // ----------------------------------------------------------------- launch ---
 
 typedef void (*Kernel)(PagedParams);
+typedef void (*Kernel2)(PagedParams, int);
 
 template <int D>
 Kernel body_kernel(int body) {
@@ -1082,11 +1140,11 @@ int MAC_PAGED_CAT(paged_resident_, MAC_PAGED_NAME)(int D, int body, int B) {
 hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, int D, int body, int grid, hipStream_t stream) {
   hipLaunchKernelGGL(body_of(D, body), dim3(grid), dim3(256), plan_bytes(p.B), stream, p);
   if (p.stream) {
-    const dim3 rows(static_cast<unsigned>(p.total_q * p.Hq));
-    const int kc = kBodyCols[body];
-    if (D == 64) hipLaunchKernelGGL((combine_kernel<64>), rows, dim3(256), 0, stream, p, kc);
-    else if (D == 128) hipLaunchKernelGGL((combine_kernel<128>), rows, dim3(256), 0, stream, p, kc);
-    else hipLaunchKernelGGL((combine_kernel<256>), rows, dim3(256), 0, stream, p, kc);
+    const bool wide = body >= kBodyTile64;
+    const dim3 rows(static_cast<unsigned>(wide ? p.total_q : p.total_q * p.Hq));
+    const Kernel2 kern = D == 64 ? (wide ? combine_rows_kernel<64> : combine_kernel<64>)
+                                 : (D == 128 ? (wide ? combine_rows_kernel<128> : combine_kernel<128>) : combine_rows_kernel<256>);
+    hipLaunchKernelGGL(kern, rows, dim3(256), 0, stream, p, kBodyCols[body]);
   }
   return hipGetLastError();
 }
