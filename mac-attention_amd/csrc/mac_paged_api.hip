@@ -28,14 +28,14 @@ bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
 
 struct Choice {
-  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = 0, grid = 0;
+  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = 0, by_rows = 0, grid = 0;
   size_t plan_bytes = 0, ml_bytes = 0, o_bytes = 0;
   size_t bytes() const { return plan_bytes + ml_bytes + o_bytes; }
 };
 
 struct Variant {
   int (*resident)(int, int, int);
-  hipError_t (*launch)(const PagedParams&, int, int, int, hipStream_t);
+  hipError_t (*launch)(const PagedParams&, int, int, hipStream_t);
 };
 
 Variant variant(int q_dtype, int cache_dtype) {
@@ -77,18 +77,23 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int64_t worst = static_cast<int64_t>(B) * ((total_q * G + ch.cols - 1) / ch.cols) * c.Hkv;
   if (worst >= INT_MAX) return false;
   const int resident = variant(q_dtype, c.cache_dtype).resident(c.D, ch.body, B);
-  // The tile body streams its keys where its tasks alone leave a quarter of the GPU
-  // idle; else workgroups that take whole tasks, in step over the same keys, share
-  // them in L2 and write no partial states.  Streamed / whole, 4 heads per group (us):
-  // 512 rows over 32K keys (128 tasks of 512 resident) 377 / 893, over 8K 149 / 240,
-  // 1024 over 8K (256) 260 / 248, 2048 over 2K (512) 208 / 83, over 8K 444 / 320; 24
-  // ragged requests, 64 dims, 592 bounding tasks of 768, 158 / 144.
-  ch.stream = ch.body <= kBodyStream32 || 4 * tasks < 3 * static_cast<int64_t>(resident);
+  // The tile body streams its keys where its tasks leave part of the GPU idle; else
+  // workgroups that take whole tasks, in step over the same keys, share them in L2 and
+  // write no partial states.  Streamed / whole, 4 heads per group (us): 512 rows over 32K
+  // keys (128 tasks of 512 resident) 354 / 893, over 8K 127 / 240, 1024 over 8K (256) 207 /
+  // 248; 24 ragged requests of 64 dims (592 tasks of 768) 106 / 140; 2048 rows over 2K (512
+  // of 512) 116 / 84, over 8K 364 / 320, 4 x 2048 of 64 dims (1024 of 768) 482 / 408.
+  ch.stream = ch.body <= kBodyStream32 || tasks < resident;
   ch.grid = resident;
   if (!ch.stream) {
     ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));
     return true;
   }
+  // Up to four pieces a task, of many rows: a wave per row and head joins them, else a
+  // workgroup.  Wave / workgroup (us): 24 ragged requests of 64 dims (1.3 pieces) 106 /
+  // 151, 512 rows of 4 heads over 32K keys (4) 373 / 389, 256 (8) 226 / 220, 128 (16) 171
+  // / 129, 64 (64) 192 / 86; a token of 256 dims over 8K (256) 144 / 33.
+  ch.by_rows = ch.body >= kBodyTile64 && ch.grid <= 4 * tasks;
   ch.unit_shift = 7 - ch.heads_shift;  // one block of each wave
   while (ch.unit_shift < 30 && (((max_keys + (int64_t{1} << ch.unit_shift) - 1) >> ch.unit_shift) + 1) * worst >= INT_MAX) ++ch.unit_shift;
   if (2 * worst >= INT_MAX || total_q * Hq > INT_MAX) return false;
@@ -201,8 +206,8 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   p.task_rows = ch.task_rows;
   p.unit_shift = ch.unit_shift;
   p.stream = ch.stream;
+  p.by_rows = ch.by_rows;
   p.grid = ch.grid;
-  p.min_units = 1;
   const double raw = a->sm_scale * c->k_scale;
   p.q_scale = static_cast<float>(a->logit_cap > 0 ? 1.0 : raw * log2e);
   p.cap_in = a->logit_cap > 0 ? static_cast<float>(2.0 * log2e * raw / a->logit_cap) : 0.0f;
@@ -213,7 +218,7 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   REQUIRE(a->logit_cap == 0 || (p.cap_in >= FLT_MIN && std::isfinite(p.cap_in) && p.cap_out >= FLT_MIN && std::isfinite(p.cap_out)),
           "logit_cap does not fit fp32 with sm_scale");
   p.v_scale = c->v_scale;
-  const hipError_t e = variant(a->q_dtype, c->cache_dtype).launch(p, c->D, ch.body, ch.grid, static_cast<hipStream_t>(stream));
+  const hipError_t e = variant(a->q_dtype, c->cache_dtype).launch(p, c->D, ch.body, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return mac::fail(MAC_ERR_HIP, "paged chunk attention: %s", hipGetErrorString(e));
   return MAC_OK;
 }

@@ -41,8 +41,8 @@ struct PagedParams {
   int task_rows;    // most rows that a task's columns touch
   int unit_shift;   // stream form; 0 units: plain form
   int stream;       // 1: stream form
-  int grid;         // workgroups of the stream form (slots hold 2 partials of each)
-  int min_units;    // least units per workgroup worth starting it for
+  int by_rows;      // stream form: 1: partial states combined a row, 0: a row and head per workgroup
+  int grid;         // workgroups (stream form: slots hold 2 partials of each)
   float q_scale;    // sm_scale k_scale log2(e); with a cap: 1 (scores are capped to log2 units)
   float cap_in, cap_out;  // 2 log2(e) sm_scale k_scale / cap, cap log2(e); 0: no cap
   float v_scale;
@@ -136,7 +136,7 @@ __device__ __forceinline__ int paged_find(const int* s_pre, int B, int x) {
 
 // Stream form: workgroups that get units, and the first unit of workgroup w.
 __device__ __forceinline__ int stream_groups(PagedArgs& p, int total) {
-  return min(p.grid, max(total / p.min_units, 1));
+  return min(p.grid, max(total, 1));
 }
 __device__ __forceinline__ int stream_begin(int w, int total, int groups) {
   return static_cast<int>(static_cast<int64_t>(w) * total / groups);
@@ -256,9 +256,9 @@ constexpr int kBodyCols[kBodies] = {16, 32, 64, 128};
 
 // Resident workgroups of a body on the current device, and its launch (with
 // the combining one in the stream form).
-#define MAC_PAGED_VARIANT_DECL(name)                                                       \
-  int paged_resident_##name(int D, int body, int B);                                       \
-  hipError_t paged_launch_##name(const PagedParams& p, int D, int body, int grid, hipStream_t stream);
+#define MAC_PAGED_VARIANT_DECL(name)                 \
+  int paged_resident_##name(int D, int body, int B); \
+  hipError_t paged_launch_##name(const PagedParams& p, int D, int body, hipStream_t stream);
 MAC_PAGED_VARIANT_DECL(bf16)
 MAC_PAGED_VARIANT_DECL(f16)
 MAC_PAGED_VARIANT_DECL(bf16_fp8)

@@ -20,8 +20,8 @@
 // a power of two is exact in bf16, and gfx950 converts two codes and applies
 // the row's scale in one instruction, so the products run as for 16-bit rows.
 // A static k_scale is part of the softmax scale, v_scale of the final
-// normalisation.  P is rounded to the queries' type for its product (2^-9 or
-// 2^-12 of each weight, as much as the output's own rounding); sums are fp32.
+// normalisation.  P is rounded to the queries' type for its product (2^-8 or
+// 2^-11 of each weight, as much as the output's own rounding); sums are fp32.
 //
 // Masked keys: keys past a row's range, past the cache or without a page get
 // s = -inf, and V of keys that no row may see is zeroed when staged.  A key that
@@ -294,15 +294,20 @@ __device__ __forceinline__ bool next_run(PagedArgs& p, const int* s_pre, int x0,
 // take different keys, 32 at a time, and meet once, at the end of a run.  Rows of
 // fewer than 256 bytes are read with their neighbours': two (four) waves take two
 // (four) KV heads of the same keys, and a token's heads, which lie side by side,
-// come from memory together (@@).  A
-// wave needs no barrier on its way: it loads whole rows (a quarter of a wave
-// reads one or two of them; operand order, a row per lane, takes eight times the
-// cache lookups per byte and ran at 4.2 TB/s where this runs at @@), and stages
-// them in tiles of LDS of its own, K as cached in XOR-swizzled chunks, V as 16-bit
-// values for the transposing reads.  A block's registers are free for the next
-// one's loads as soon as it is staged, so those are in flight while it is
-// computed; their page entries went out a block before.
-constexpr int kOddBlocks = 8;  // a wave's blocks at the rows' edges: a task has at most 32 rows, so 63 keys at either end
+// come from memory together (64 requests over 26K 8-bit keys of 8 heads of 128 dims
+// 645 -> 600 us).  A wave needs no barrier on its way: it loads whole rows (a
+// quarter of a wave reads one or two of them; operand order, a row per lane, takes
+// eight times the cache lookups per byte and ran at 4.2 TB/s where this runs at
+// 6.1), and stages them in tiles of LDS of its own, K as cached in XOR-swizzled
+// chunks, V as 16-bit values for the transposing reads.  A block's registers are
+// free for the next one's loads as soon as it is staged, so those are in flight
+// while it is computed (a second block in flight, of 8-bit rows: 595 -> 643 us, for
+// the registers); their page entries went out a block before.
+//
+// A wave's blocks that hold keys which only some rows see: a task has at most 32
+// rows, so 31 such keys at either end, 2 blocks each (3 in all under a window
+// shorter than that).
+constexpr int kOddBlocks = 4;
 
 template <int D, int kPer>
 __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
@@ -314,7 +319,6 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   constexpr int kVU = D / 8 + 2;            // 16-byte units per staged V row
   constexpr int kDT = D / 16;
   constexpr int kC = 16 * kPer;
-  constexpr int kSets = 1;  // blocks in flight (two, of 8-bit rows: 643 us where one takes 595)
   constexpr int kOut = D + 4;               // floats per column of the joined state
   extern __shared__ int s_pre[];
   __shared__ int s_tmp[4];
@@ -380,16 +384,16 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
     const char* const kb = p.k + at64(hkv, p.kv_hs) + 16 * ld_ch;
     const int64_t v_minus_k = p.v - p.k;
     const int last_entry = p.table_cols - 1;
-    // the blocks in flight
+    // the block in flight
     struct Flight {
       pa_u32x4 k[kNI], v[kNI];
       uint32_t sc, bad;  // scale bytes of key lane % 32, keys without a row
     };
-    Flight flight[kSets];
+    Flight fl;
     auto entry = [&](int base) {
       return t.table[static_cast<uint32_t>(min((base + (lane & 31)) >> page_shift, last_entry))];
     };
-    auto load = [&](int base, int e, Flight& fl) {
+    auto load = [&](int base, int e) {
       const int key = base + (lane & 31);
       const bool ok = key < t.khi && static_cast<uint32_t>(e) < num_pages;
       fl.bad = ~static_cast<uint32_t>(__ballot(ok));
@@ -415,21 +419,15 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
 
     bool far = false;
     int n_odd = 0;  // blocks in s_odd
-    // the wave's blocks: every fourth of the run's (of two
-    // heads: every second).  Blocks past it are loaded
-    // too (the cache's first page): behind a branch their number would be unknown
-    // to the waits for the blocks before them.
+    // the wave's blocks: every fourth of the run's (of two heads: every second)
     int base = t.klo + 32 * (wave >> heads_shift);
     int e_next = 0;  // entries of the block to load next
     if (base < t.khi) {
-#pragma unroll
-      for (int i = 0; i < kSets; ++i) {
-        const int e = entry(base + key_step * i);
-        if (i == kSets - 1) e_next = entry(base + key_step * kSets);
-        load(base + key_step * i, e, flight[i]);
-      }
+      const int e = entry(base);
+      e_next = entry(base + key_step);
+      load(base, e);
     }
-    auto step = [&](Flight& fl) {
+    auto step = [&]() {  // (written out in the loop, rows of 64 bytes took 488 us for 432)
       const uint32_t bad = __builtin_amdgcn_readfirstlane(fl.bad);
       const bool part = base < all_lo || base + 32 > all_hi;  // some row of the task does not see some key
       const bool masked = part || bad != 0;
@@ -471,9 +469,9 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_sched_barrier(0);
-      if (kSets > 1 || base + key_step * kSets < t.khi) {
-        const int e_after = entry(base + key_step * (kSets + 1));  // (ahead of the rows: the wait for it is no wait for them)
-        load(base + key_step * kSets, e_next, fl);
+      if (base + key_step < t.khi) {
+        const int e_after = entry(base + 2 * key_step);  // (ahead of the rows: the wait for it is no wait for them)
+        load(base + key_step, e_next);
         e_next = e_after;
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -530,13 +528,8 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
       }
     };
     while (base < t.khi) {
-      step(flight[0]);
+      step();
       base += key_step;
-      if constexpr (kSets > 1) {
-        if (base >= t.khi) break;
-        step(flight[1]);
-        base += key_step;
-      }
     }
 
     PagedArgs& e = fresh_args();
@@ -1011,8 +1004,8 @@ __device__ __forceinline__ Joined<kV> join_pieces(PagedArgs& p, const Pieces& x,
   return s;
 }
 
-// Few rows, each in many pieces (stream body): one workgroup per (row, query
-// head), its waves take every fourth piece.
+// Rows in many pieces: one workgroup per (row, query head), its waves take every
+// fourth piece.
 template <int D>
 __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   PagedArgs& p = fresh_args();
@@ -1058,8 +1051,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   if (tid == 0) p.lse[at] = lt == 0.0f ? -INFINITY : (mx + fast_log2(lt)) * kLn2;
 }
 
-// Many rows in few pieces (tile body): one workgroup per row, a wave per query
-// head in turn.
+// Rows in few pieces: one workgroup per row, a wave per query head in turn.
 template <int D>
 __global__ void __launch_bounds__(256) combine_rows_kernel(PagedParams, int kc) {
   PagedArgs& p = fresh_args();
@@ -1107,6 +1099,10 @@ Kernel body_kernel(int body) {
 Kernel body_of(int D, int body) {
   return D == 64 ? body_kernel<64>(body) : (D == 128 ? body_kernel<128>(body) : body_kernel<256>(body));
 }
+template <int D>
+Kernel2 combine_of(bool by_rows) {
+  return by_rows ? combine_rows_kernel<D> : combine_kernel<D>;
+}
 size_t plan_bytes(int B) { return sizeof(int) * (static_cast<size_t>(B) + 1); }
 
 }  // namespace
@@ -1137,14 +1133,12 @@ int MAC_PAGED_CAT(paged_resident_, MAC_PAGED_NAME)(int D, int body, int B) {
   return cus * per;
 }
 
-hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, int D, int body, int grid, hipStream_t stream) {
-  hipLaunchKernelGGL(body_of(D, body), dim3(grid), dim3(256), plan_bytes(p.B), stream, p);
+hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, int D, int body, hipStream_t stream) {
+  hipLaunchKernelGGL(body_of(D, body), dim3(p.grid), dim3(256), plan_bytes(p.B), stream, p);
   if (p.stream) {
-    const bool wide = body >= kBodyTile64;
-    const dim3 rows(static_cast<unsigned>(wide ? p.total_q : p.total_q * p.Hq));
-    const Kernel2 kern = D == 64 ? (wide ? combine_rows_kernel<64> : combine_kernel<64>)
-                                 : (D == 128 ? (wide ? combine_rows_kernel<128> : combine_kernel<128>) : combine_rows_kernel<256>);
-    hipLaunchKernelGGL(kern, rows, dim3(256), 0, stream, p, kBodyCols[body]);
+    const Kernel2 kern = D == 64 ? combine_of<64>(p.by_rows) : (D == 128 ? combine_of<128>(p.by_rows) : combine_of<256>(p.by_rows));
+    const unsigned grid = static_cast<unsigned>(p.by_rows ? p.total_q : p.total_q * p.Hq);
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, stream, p, kBodyCols[body]);
   }
   return hipGetLastError();
 }

@@ -1026,7 +1026,7 @@ _ANY_WINDOW = 1 << 30  # a window that covers every key of any request
 # well (get_device() is -1 off the GPU), its message comes from a second look, and
 # the argument blocks are packed in one call instead of field by field (a decode
 # batch's write 13.7 us a call with ctypes structures and a device object per
-# tensor, @W now; a decode step of one request 24.2 and @A).
+# tensor, 10.2 now; a decode step of one request 24.2 and 19.1).
 
 
 def _packer(cls: type, fmt: str):
