@@ -28,7 +28,7 @@ bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15)
 constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
 
 struct Choice {
-  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = 0, by_rows = 0, grid = 0;
+  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = kPlain, by_rows = 0, grid = 0;
   size_t plan_bytes = 0, ml_bytes = 0, o_bytes = 0;
   size_t bytes() const { return plan_bytes + ml_bytes + o_bytes; }
 };
@@ -83,9 +83,17 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   // keys (128 tasks of 512 resident) 354 / 893, over 8K 127 / 240, 1024 over 8K (256) 207 /
   // 248; 24 ragged requests of 64 dims (592 tasks of 768) 106 / 140; 2048 rows over 2K (512
   // of 512) 116 / 84, over 8K 364 / 320, 4 x 2048 of 64 dims (1024 of 768) 482 / 408.
-  ch.stream = ch.body <= kBodyStream32 || tasks < resident;
+  // The tasks of one request are about as long as each other; of several, the device
+  // looks (paged_plan).
+  const bool fits = 2 * worst < INT_MAX;  // (the units of a task and its partial states)
+  if (ch.body <= kBodyStream32 || tasks < resident) {
+    if (!fits) return false;
+    ch.stream = kStream;
+  } else {
+    ch.stream = B > 1 && fits ? kEither : kPlain;
+  }
   ch.grid = resident;
-  if (!ch.stream) {
+  if (ch.stream == kPlain) {
     ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));
     return true;
   }
@@ -96,8 +104,7 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   ch.by_rows = ch.body >= kBodyTile64 && ch.grid <= 4 * tasks;
   ch.unit_shift = 7 - ch.heads_shift;  // one block of each wave
   while (ch.unit_shift < 30 && (((max_keys + (int64_t{1} << ch.unit_shift) - 1) >> ch.unit_shift) + 1) * worst >= INT_MAX) ++ch.unit_shift;
-  if (2 * worst >= INT_MAX || total_q * Hq > INT_MAX) return false;
-  ch.plan_bytes = up16(sizeof(int) * (static_cast<size_t>(B) + 1));
+  ch.plan_bytes = up16(sizeof(int) * (static_cast<size_t>(B) + 2));
   const size_t slots = 2 * static_cast<size_t>(ch.grid) * (room << ch.heads_shift);
   ch.ml_bytes = slots * 2 * sizeof(float);
   ch.o_bytes = slots * c.D * sizeof(float);
@@ -178,7 +185,7 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   p.req_ids = a->req_ids;
   p.out = static_cast<uint16_t*>(a->out);
   p.lse = a->out_lse;
-  if (ch.stream) {
+  if (ch.stream != kPlain) {
     char* w = static_cast<char*>(workspace);
     p.plan = reinterpret_cast<int32_t*>(w);
     p.part_ml = reinterpret_cast<float*>(w + ch.plan_bytes);

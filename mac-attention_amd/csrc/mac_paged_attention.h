@@ -10,6 +10,10 @@
 
 namespace mac {
 
+// Plain form: workgroups take whole tasks in turn.  kEither: the device decides, from
+// the lengths that the host does not know (paged_plan).
+enum { kPlain = 0, kStream = 1, kEither = 2 };
+
 // What the kernels read.  A call's queries are cut into tasks of `cols`
 // (row, head) columns of one request and KV head; stream form: the tasks' keys
 // laid end to end in units of 2^unit_shift keys, dealt to the workgroups in
@@ -27,7 +31,7 @@ struct PagedParams {
   float* lse;
   float* part_o;   // stream form: [2 grid][heads][body's columns][D] unnormalised partial outputs
   float* part_ml;  // [2 grid][heads][columns][2] their reference points (log2 units) and sums
-  int32_t* plan;   // [B + 1] units before each request, for the combining launch
+  int32_t* plan;   // [B + 1] units before each request, for the combining launch; whether there are any
   int64_t q_ts, q_hs;                          // elements
   uint32_t kv_ps, kv_ss, kv_hs;  // bytes: page, slot and head strides of K and of V
   int64_t table_stride;
@@ -39,8 +43,8 @@ struct PagedParams {
   int cols;         // columns of a task per KV head (whole rows where a row's heads fit one)
   int heads_shift;  // a task takes 2^heads_shift KV heads (stream body)
   int task_rows;    // most rows that a task's columns touch
-  int unit_shift;   // stream form; 0 units: plain form
-  int stream;       // 1: stream form
+  int unit_shift;   // stream form
+  int stream;       // kPlain, kStream or kEither
   int by_rows;      // stream form: 1: partial states combined a row, 0: a row and head per workgroup
   int grid;         // workgroups (stream form: slots hold 2 partials of each)
   float q_scale;    // sm_scale k_scale log2(e); with a cap: 1 (scores are capped to log2 units)
@@ -83,20 +87,18 @@ __device__ __forceinline__ PagedRequest paged_request(PagedArgs& p, int b) {
   return r;
 }
 
-// Units (stream form) or tasks (plain form) of a request.
-__device__ __forceinline__ int paged_weight(PagedArgs& p, const PagedRequest& r) {
-  return r.tasks * (p.Hkv >> p.heads_shift) * (p.stream ? r.units : 1);
-}
-
-// Exclusive prefix of the requests' weights in s_pre[B + 1], by a workgroup of
-// 256 threads; ends with a barrier.  s_tmp: 4 entries.
-__device__ __forceinline__ void paged_plan(PagedArgs& p, int* s_pre, int* s_tmp) {
+// Exclusive prefix of the requests' units (stream form) or tasks (plain form) in
+// s_pre[B + 1], by a workgroup of 256 threads; ends with a barrier.  s_tmp: 4
+// entries.  Returns the units of the thread's longest task.
+__device__ __forceinline__ int paged_prefix(PagedArgs& p, bool stream, int* s_pre, int* s_tmp) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = ceil_div(p.B, 256);
   const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-  int sum = 0;
+  int sum = 0, longest = 0;
   for (int b = b0; b < b1; ++b) {
-    const int w = paged_weight(p, paged_request(p, b));
+    const PagedRequest r = paged_request(p, b);
+    const int w = r.tasks * (p.Hkv >> p.heads_shift) * (stream ? r.units : 1);
+    if (w != 0) longest = max(longest, r.units);
     s_pre[b] = w;
     sum += w;
   }
@@ -121,6 +123,26 @@ __device__ __forceinline__ void paged_plan(PagedArgs& p, int* s_pre, int* s_tmp)
   }
   if (tid == 0) s_pre[p.B] = total;
   __syncthreads();
+  return longest;
+}
+
+// The prefix, and the form: where a choice is left, the stream form if a task is
+// longer than a workgroup's share of the units.  Every workgroup decides alike.  Plain /
+// streamed, 8 KV heads of 4 query heads (us): a chunk of 2048 rows over its own keys and
+// one token over 128K 3365 / 299, and 63 tokens over 16K (a task is as long as the share)
+// 593 / 716; 5 requests of 512 rows over 4K to 32K 990 / 750, 12 such 1717 / 1839.
+template <bool kEitherForm>
+__device__ __forceinline__ bool paged_plan(PagedArgs& p, int* s_pre, int* s_tmp) {
+  if constexpr (!kEitherForm) {
+    paged_prefix(p, true, s_pre, s_tmp);
+    return true;
+  }
+  const int longest = paged_prefix(p, p.stream != kPlain, s_pre, s_tmp);
+  if (p.stream != kEither) return p.stream == kStream;
+  const int total = s_pre[p.B];
+  if (__syncthreads_or(static_cast<int64_t>(longest) * p.grid > total)) return true;
+  paged_prefix(p, false, s_pre, s_tmp);
+  return false;
 }
 
 // Largest b < B with pre[b] <= x.

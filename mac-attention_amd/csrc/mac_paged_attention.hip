@@ -246,9 +246,9 @@ struct Run {
 // workgroups would take the longer tasks of each (4 x 4096 rows 826 -> 777 us; a last,
 // partial round goes to the first workgroups, which a CU serves first: 4 x 2048 rows of
 // 64 dims 468 -> 413).  False: no more.
-__device__ __forceinline__ bool next_run(PagedArgs& p, const int* s_pre, int x0, int x1, int& x, Run& r) {
+__device__ __forceinline__ bool next_run(PagedArgs& p, bool stream, const int* s_pre, int x0, int x1, int& x, Run& r) {
   int at = x;
-  if (!p.stream) {
+  if (!stream) {
     const int grid = gridDim.x, w = blockIdx.x;
     const int64_t round = static_cast<int64_t>(x) * grid;
     const bool back = (x & 1) && grid % 8 == 0 && round + grid <= x1;
@@ -268,7 +268,7 @@ __device__ __forceinline__ bool next_run(PagedArgs& p, const int* s_pre, int x0,
   q.tasks = __builtin_amdgcn_readfirstlane(q.tasks);
   q.units = __builtin_amdgcn_readfirstlane(q.units);
   at -= __builtin_amdgcn_readfirstlane(s_pre[b]);
-  if (!p.stream) {
+  if (!stream) {
     const int index = at / p.Hkv, h = at - index * p.Hkv;
     r.task = paged_task(p, b, q, h * q.tasks + (q.tasks - 1 - index));
     r.whole = true;
@@ -332,7 +332,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
   PagedArgs& a0 = fresh_args();
-  paged_plan(a0, s_pre, s_tmp);
+  paged_plan<false>(a0, s_pre, s_tmp);
   const int total = __builtin_amdgcn_readfirstlane(s_pre[a0.B]);
   const int groups = stream_groups(a0, total);
   if (blockIdx.x == 0)
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
 
   int x = x0;
   Run run;
-  while (next_run(fresh_args(), s_pre, x0, x1, x, run)) {
+  while (next_run(fresh_args(), true, s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
     PagedArgs& p = fresh_args();
     const int hkv = t.hkv + own_head;
@@ -644,13 +644,15 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lane = tid & 63, quad = lane >> 4, col = lane & 15;
   PagedArgs& a0 = fresh_args();
-  paged_plan(a0, s_pre, s_tmp);
+  const bool stream = paged_plan<true>(a0, s_pre, s_tmp);
   const int total = __builtin_amdgcn_readfirstlane(s_pre[a0.B]);
   int x0 = 0, x1 = total;
-  if (a0.stream) {
+  if (a0.stream != kPlain && blockIdx.x == 0) {
+    for (int b = tid; b <= a0.B; b += 256) a0.plan[b] = s_pre[b];
+    if (tid == 0) a0.plan[a0.B + 1] = stream;
+  }
+  if (stream) {
     const int groups = stream_groups(a0, total);
-    if (blockIdx.x == 0)
-      for (int b = tid; b <= a0.B; b += 256) a0.plan[b] = s_pre[b];
     if (static_cast<int>(blockIdx.x) >= groups) return;
     x0 = stream_begin(blockIdx.x, total, groups);
     x1 = stream_begin(blockIdx.x + 1, total, groups);
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
 
   int x = x0;
   Run run;
-  while (next_run(fresh_args(), s_pre, x0, x1, x, run)) {
+  while (next_run(fresh_args(), stream, s_pre, x0, x1, x, run)) {
     const PagedTask& t = run.task;
     PagedArgs& p = fresh_args();
     const float scale = p.q_scale;
@@ -1058,6 +1060,7 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(PagedParams, int kc) 
   constexpr int kV = D / 64;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (p.plan[p.B + 1] == 0) return;  // plain form
   const int row = blockIdx.x;
   const int b = request_of_row(p, row);
   if (b < 0) return;
@@ -1135,7 +1138,7 @@ int MAC_PAGED_CAT(paged_resident_, MAC_PAGED_NAME)(int D, int body, int B) {
 
 hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, int D, int body, hipStream_t stream) {
   hipLaunchKernelGGL(body_of(D, body), dim3(p.grid), dim3(256), plan_bytes(p.B), stream, p);
-  if (p.stream) {
+  if (p.stream != kPlain) {
     const Kernel2 kern = D == 64 ? combine_of<64>(p.by_rows) : (D == 128 ? combine_of<128>(p.by_rows) : combine_of<256>(p.by_rows));
     const unsigned grid = static_cast<unsigned>(p.by_rows ? p.total_q : p.total_q * p.Hq);
     hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, stream, p, kBodyCols[body]);

@@ -106,6 +106,40 @@ def test_whole_prompts(ext, rows):
     p.check(p.run(ext))
 
 
+@pytest.mark.parametrize("window", [-1, 300])
+@pytest.mark.parametrize("lens", [[1600, 40000, 900], [1600, 1, 0], [1700, 9000, 1601], [50000, 700, 3]])
+def test_chunks_beside_single_tokens(ext, lens, window):
+    """More tasks than resident workgroups, of lengths that only the device knows: of
+    whole tasks, or streamed where one is much longer."""
+    p = Problem([1600, 1, 1], lens, 64, 8, 64, 16, "fp8", window=window, seed=lens[1])
+    p.check(p.run(ext))
+
+
+def test_captured_while_the_longest_task_changes(ext):
+    """Replays of one capture switch between whole and streamed tasks."""
+    cases = [[1600, 40000], [1600, 900], [1600, 30000], [1600, 1]]
+    p = Problem([1600, 1], cases[0], 64, 8, 64, 16, "fp8", seed=3)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        p.run(ext)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = p.run(ext)
+    for lens in cases + cases:
+        p.lens = lens
+        p.kv_lens.copy_(_i32(lens))
+        eager = [x.clone() for x in p.run(ext)]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(got, eager):
+            assert torch.equal(x, y)
+    p.lens = cases[2]
+    p.kv_lens.copy_(_i32(p.lens))
+    graph.replay()
+    p.check(got)
+
+
 def test_many_requests(ext):
     """More requests than a workgroup has threads, some without rows."""
     g = torch.Generator().manual_seed(1)
