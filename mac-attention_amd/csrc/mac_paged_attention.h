@@ -156,16 +156,23 @@ __device__ __forceinline__ int paged_find(const int* s_pre, int B, int x) {
   return lo;
 }
 
-// Stream form: workgroups that get units, and the first unit of workgroup w.
-__device__ __forceinline__ int stream_groups(PagedArgs& p, int total) {
-  return min(p.grid, max(total, 1));
-}
-__device__ __forceinline__ int stream_begin(int w, int total, int groups) {
-  return static_cast<int>(static_cast<int64_t>(w) * total / groups);
-}
-// The workgroup whose run holds unit x.
-__device__ __forceinline__ int stream_owner(int x, int total, int groups) {
-  return static_cast<int>((static_cast<int64_t>(x + 1) * groups + total - 1) / total) - 1;
+// Stream form: the units dealt to the workgroups in equal runs, the first `more` of
+// them with one unit more.
+struct Deal {
+  uint32_t groups, each, more;
+  __device__ __forceinline__ int begin(uint32_t w) const { return static_cast<int>(w * each + min(w, more)); }
+  // the workgroup whose run holds unit x
+  __device__ __forceinline__ int owner(uint32_t x) const {
+    const uint32_t longer = more * (each + 1);
+    return static_cast<int>(x < longer ? x / (each + 1) : more + (x - longer) / each);
+  }
+};
+__device__ __forceinline__ Deal stream_deal(PagedArgs& p, int total) {
+  Deal d;
+  d.groups = min(p.grid, max(total, 1));
+  d.each = static_cast<uint32_t>(total) / d.groups;
+  d.more = total - d.each * d.groups;
+  return d;
 }
 
 // One of a task's runs of keys.

@@ -334,11 +334,11 @@ __global__ void __launch_bounds__(256, 2) stream_kernel(PagedParams) {
   PagedArgs& a0 = fresh_args();
   paged_plan<false>(a0, s_pre, s_tmp);
   const int total = __builtin_amdgcn_readfirstlane(s_pre[a0.B]);
-  const int groups = stream_groups(a0, total);
+  const Deal deal = stream_deal(a0, total);
   if (blockIdx.x == 0)
     for (int b = tid; b <= a0.B; b += 256) a0.plan[b] = s_pre[b];
-  if (static_cast<int>(blockIdx.x) >= groups) return;
-  const int x0 = stream_begin(blockIdx.x, total, groups), x1 = stream_begin(blockIdx.x + 1, total, groups);
+  if (blockIdx.x >= deal.groups) return;
+  const int x0 = deal.begin(blockIdx.x), x1 = deal.begin(blockIdx.x + 1);
 
   // chunk c of staged K row r lies at c ^ swizzle(r): eight rows' chunks on different banks
   auto swizzle = [](int r) { return kRL >= 16 ? r & 15 : (kRL == 8 ? r & 7 : (r >> 2) & 3); };
@@ -652,10 +652,10 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
     if (tid == 0) a0.plan[a0.B + 1] = stream;
   }
   if (stream) {
-    const int groups = stream_groups(a0, total);
-    if (static_cast<int>(blockIdx.x) >= groups) return;
-    x0 = stream_begin(blockIdx.x, total, groups);
-    x1 = stream_begin(blockIdx.x + 1, total, groups);
+    const Deal deal = stream_deal(a0, total);
+    if (blockIdx.x >= deal.groups) return;
+    x0 = deal.begin(blockIdx.x);
+    x1 = deal.begin(blockIdx.x + 1);
   }
   // loader: thread t stages chunk t % kRowCh of keys t / kRowCh + kStep i
   const int ld_key = tid / kRowCh, ld_ch = tid % kRowCh;
@@ -941,25 +941,24 @@ __global__ void __launch_bounds__(256, kOcc) tile_kernel(PagedParams) {
 struct Pieces {
   int first, n;
   bool at_start;  // the first one's run begins with the task
-  int64_t offset;  // of the column in a slot
+  int offset;      // of the column in a slot
   __device__ __forceinline__ int64_t place(int i, int64_t slot_columns) const {
     const int64_t slot = 2 * static_cast<int64_t>(first + i) + (i == 0 && !at_start ? 1 : 0);
     return slot * slot_columns + offset;
   }
 };
-__device__ __forceinline__ Pieces find_pieces(PagedArgs& p, const PagedRequest& r, int before, int total, int row, int head, int kc) {
-  const int groups = stream_groups(p, total);
+__device__ __forceinline__ Pieces find_pieces(PagedArgs& p, const PagedRequest& r, int before, const Deal& deal, int row, int head, int kc) {
   const int hkv = head / p.G;
   const int gc = (row - r.q0) * p.G + head - hkv * p.G;
   const int ct = gc / p.cols, col = gc - ct * p.cols;
   const int group = hkv >> p.heads_shift;
   const int unit = before + (group * r.tasks + ct) * r.units;
   Pieces x;
-  x.first = stream_owner(unit, total, groups);
-  x.n = stream_owner(unit + r.units - 1, total, groups) - x.first;
+  x.first = deal.owner(unit);
+  x.n = deal.owner(unit + r.units - 1) - x.first;
   x.n = x.n > 0 ? x.n + 1 : 0;
-  x.at_start = stream_begin(x.first, total, groups) == unit;
-  x.offset = static_cast<int64_t>(hkv - (group << p.heads_shift)) * kc + col;
+  x.at_start = deal.begin(x.first) == unit;
+  x.offset = (hkv - (group << p.heads_shift)) * kc + col;
   return x;
 }
 // The request that a row belongs to (-1: none), for a whole workgroup.
@@ -1020,7 +1019,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   if (b < 0) return;
   const PagedRequest r = paged_request(p, b);
   if (r.n == 0) return;
-  const Pieces x = find_pieces(p, r, p.plan[b], p.plan[p.B], row, head, kc);
+  const Pieces x = find_pieces(p, r, p.plan[b], stream_deal(p, p.plan[p.B]), row, head, kc);
   if (x.n == 0) return;  // stored by its workgroup
   const Joined<kV> s = join_pieces<kV>(p, x, static_cast<int64_t>(kc) << p.heads_shift, wave, 4);
 #pragma unroll
@@ -1053,7 +1052,8 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   if (tid == 0) p.lse[at] = lt == 0.0f ? -INFINITY : (mx + fast_log2(lt)) * kLn2;
 }
 
-// Rows in few pieces: one workgroup per row, a wave per query head in turn.
+// Rows in few pieces: gridDim.y workgroups per row, a wave per query head in turn;
+// 64 heads' pieces are looked up together, one in a lane.
 template <int D>
 __global__ void __launch_bounds__(256) combine_rows_kernel(PagedParams, int kc) {
   PagedArgs& p = fresh_args();
@@ -1066,10 +1066,18 @@ __global__ void __launch_bounds__(256) combine_rows_kernel(PagedParams, int kc) 
   if (b < 0) return;
   const PagedRequest r = paged_request(p, b);
   if (r.n == 0) return;
-  const int before = p.plan[b], total = p.plan[p.B];
-  for (int head = wave; head < p.Hq; head += 4) {
-    const Pieces x = find_pieces(p, r, before, total, row, head, kc);
+  const int before = p.plan[b];
+  const Deal deal = stream_deal(p, p.plan[p.B]);
+  const int step = 4 * gridDim.y;
+  Pieces found = {};
+  for (int i = 0, head = 4 * blockIdx.y + wave; head < p.Hq; ++i, head += step) {
+    if (i % 64 == 0) found = find_pieces(p, r, before, deal, row, min(head + step * lane, p.Hq - 1), kc);
+    Pieces x;
+    x.n = __builtin_amdgcn_readlane(found.n, i % 64);
     if (x.n == 0) continue;
+    x.first = __builtin_amdgcn_readlane(found.first, i % 64);
+    x.at_start = __builtin_amdgcn_readlane(found.at_start, i % 64);
+    x.offset = __builtin_amdgcn_readlane(found.offset, i % 64);
     const Joined<kV> s = join_pieces<kV>(p, x, static_cast<int64_t>(kc) << p.heads_shift, 0, 1);
     const int64_t at = static_cast<int64_t>(row) * p.Hq + head;
     const float inv = s.l == 0.0f ? 0.0f : p.v_scale / s.l;
@@ -1140,8 +1148,10 @@ hipError_t MAC_PAGED_CAT(paged_launch_, MAC_PAGED_NAME)(const PagedParams& p, in
   hipLaunchKernelGGL(body_of(D, body), dim3(p.grid), dim3(256), plan_bytes(p.B), stream, p);
   if (p.stream != kPlain) {
     const Kernel2 kern = D == 64 ? combine_of<64>(p.by_rows) : (D == 128 ? combine_of<128>(p.by_rows) : combine_of<256>(p.by_rows));
-    const unsigned grid = static_cast<unsigned>(p.by_rows ? p.total_q : p.total_q * p.Hq);
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(256), 0, stream, p, kBodyCols[body]);
+    const unsigned rows = static_cast<unsigned>(p.total_q), heads = p.Hq;
+    // (few rows: their heads spread over more workgroups)
+    const dim3 grid = p.by_rows ? dim3(rows, std::clamp(1024u / rows, 1u, (heads + 3) / 4)) : dim3(rows * heads);
+    hipLaunchKernelGGL(kern, grid, dim3(256), 0, stream, p, kBodyCols[body]);
   }
   return hipGetLastError();
 }
