@@ -412,7 +412,7 @@ typedef struct MacPagedCache {
  * i64); locs outside the cache (negative: padding) are skipped.  Row-scaled
  * form: the row's scale is the smallest power of two s >= 2^-126 with max |x|
  * <= 448 s over its finite elements; static form: x / k_scale, saturated.
- * Codes round to nearest even; NaN and infinities become NaN.  D: multiples of
+ * Codes round to nearest even; NaN and infinities in k and v become NaN.  D: multiples of
  * 16 up to 256.  Two tokens of one call must not name the same slot: its row
  * and scale would be one token's or the other's, element by element. */
 MAC_API int mac_paged_cache_write_fp8(const MacPagedCache* cache, const void* k, int64_t k_stride0, int64_t k_stride1,
@@ -422,7 +422,8 @@ MAC_API int mac_paged_cache_write_fp8(const MacPagedCache* cache, const void* k,
 
 /* Decode RoPE with that write (the 8-bit counterpart of
  * mac_decode_rope_preserve_q_bf16): q_out[n] = RoPE(q[n]) ([tokens, Hq, D],
- * contiguous, 16-byte aligned; q itself is left as it is, the pre-RoPE query),
+ * contiguous, 16-byte aligned; q itself is left as it is, the pre-RoPE query,
+ * and q_out must overlap neither it nor k and v),
  * and RoPE(k[n]) (fp32, quantised without another rounding) and v[n] go to
  * slot cache_locs[n].  RoPE, cos_sin_cache, positions and is_neox as in
  * mac_decode_rope_preserve_q_bf16. */
@@ -448,9 +449,9 @@ MAC_API int mac_paged_rope_write_fp8(const MacPagedCache* cache, const MacPagedR
 
 /* Reads rows back: out_k[i], out_v[i] ([rows, Hkv, D] of dtype MAC_DTYPE_F32 /
  * BF16 / F16, contiguous, 16-byte aligned) are the values of slot
- * kv_indices[i]; slots outside the cache read as zeros.  Exact in fp32 and,
- * row-scaled, in bf16 (subnormals of 2^-126 scales aside); otherwise rounded to
- * nearest even. */
+ * kv_indices[i]; slots outside the cache read as zeros.  Row-scaled: exact in
+ * fp32 and (subnormals of 2^-126 scales aside) in bf16; static form: the fp32
+ * product; rounded to nearest even where dtype has fewer bits. */
 MAC_API int mac_paged_cache_read_fp8(const MacPagedCache* cache, const void* kv_indices, int32_t kv_indices_is_i64,
                                      int64_t rows, void* out_k, void* out_v, int32_t dtype, void* stream);
 
@@ -481,7 +482,7 @@ MAC_API int mac_paged_cache_read_fp8(const MacPagedCache* cache, const void* kv_
  * weights, as in a softmax over them); in keys that it does not see they do not.
  * Sums are fp32; weights are rounded to q_dtype for their product with V.  A
  * call's results depend on its inputs, shapes and the device only.  At most 4096
- * requests.
+ * requests, fewer than 2^24 query rows and 2^31 (row, head) pairs.
  */
 typedef struct MacPagedAttentionArgs {
   uint32_t struct_size; /* sizeof(MacPagedAttentionArgs) */

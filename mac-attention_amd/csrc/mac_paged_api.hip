@@ -26,6 +26,7 @@ using namespace mac;
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
 
 constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
+constexpr int kMaxQ = 1 << 24;  // workgroups: a launch has fewer than 2^32 threads
 
 struct Choice {
   int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = kPlain, by_rows = 0, grid = 0;
@@ -102,6 +103,7 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   // 151, 512 rows of 4 heads over 32K keys (4) 373 / 389, 256 (8) 226 / 220, 128 (16) 171
   // / 129, 64 (64) 192 / 86; a token of 256 dims over 8K (256) 144 / 33.
   ch.by_rows = ch.body >= kBodyTile64 && ch.grid <= 4 * tasks;
+  if (!ch.by_rows && total_q * Hq >= kMaxQ) return false;
   ch.unit_shift = 7 - ch.heads_shift;  // one block of each wave
   while (ch.unit_shift < 30 && (((max_keys + (int64_t{1} << ch.unit_shift) - 1) >> ch.unit_shift) + 1) * worst >= INT_MAX) ++ch.unit_shift;
   ch.plan_bytes = up16(sizeof(int) * (static_cast<size_t>(B) + 2));
@@ -122,7 +124,7 @@ int check(const MacPagedCache* c, const MacPagedAttentionArgs* a) {
   REQUIRE(c->D == 64 || c->D == 128 || c->D == 256, "head_dim must be 64, 128 or 256 (got %d)", c->D);
   REQUIRE(a->Hq > 0 && c->Hkv > 0 && a->Hq % c->Hkv == 0, "Hq must be a positive multiple of Hkv");
   REQUIRE(a->B >= 0 && a->B <= kMaxB, "B must be in [0, %d] (got %d)", kMaxB, a->B);
-  REQUIRE(a->total_q >= 0 && a->total_q <= INT_MAX / a->Hq, "total_q too large");
+  REQUIRE(a->total_q >= 0 && a->total_q < kMaxQ && a->total_q <= INT_MAX / a->Hq, "total_q too large");
   REQUIRE(c->num_pages > 0 && c->num_pages <= INT_MAX, "num_pages must be positive (and fit 31 bits)");
   REQUIRE(c->page_size > 0 && (c->page_size & (c->page_size - 1)) == 0, "page_size must be a power of two (got %d)",
           c->page_size);

@@ -19,10 +19,15 @@
 // group, four conversions, one 8-byte store.  K and V rows of a (token, head)
 // go together, so both scale bytes leave in one 2-byte store.  The kernels are
 // bound by their bytes (or, for a decode batch, by the launch): a lane has all
-// of its loads in flight at once and there is no loop.
+// of its loads in flight at once and there is no loop.  Measured, 8 KV heads of
+// 128 dims: 32768 tokens written in 43 us (4.7 TB/s where a device copy reaches
+// 4.9), 65536 read back to bf16 in 80 (5.1 TB/s); RoPE with the write, 32 query
+// heads, 2048 tokens 15 us from a warm cache (3.1 TB/s); 64 tokens, either write, 4
+// to 5 us.
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -134,11 +139,12 @@ __device__ __forceinline__ uint32_t scale_byte(float amax) {
   return static_cast<uint32_t>(max(e, 1));
 }
 
-// Codes of eight elements y (already divided by their scale).
-__device__ __forceinline__ uint2 encode8(const float (&y)[8]) {
+// Codes of eight elements x whose quotients by their scale are y (infinite where a
+// static scale is too small: those saturate).
+__device__ __forceinline__ uint2 encode8(const float (&x)[8], const float (&y)[8]) {
   float c[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = finite(y[i]) ? fminf(fmaxf(y[i], -kTop), kTop) : __uint_as_float(0x7fc00000u);
+  for (int i = 0; i < 8; ++i) c[i] = finite(x[i]) ? fminf(fmaxf(y[i], -kTop), kTop) : __uint_as_float(0x7fc00000u);
   int lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
   lo = __builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], lo, true);
   int hi = __builtin_amdgcn_cvt_pk_fp8_f32(c[4], c[5], 0, false);
@@ -160,7 +166,7 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], bool scaled, flo
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(x[i], factor);
   }
-  return encode8(y);
+  return encode8(x, y);
 }
 
 // Stores a (token, head)'s lane: codes of K and V and the scale bytes.  Locs
@@ -356,6 +362,14 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(CacheParams p) {
 bool aligned(const void* ptr, int n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1)) == 0; }
 bool vec16(const void* ptr, int64_t ts, int64_t hs) { return aligned(ptr, 16) && ((ts | hs) & 7) == 0; }
 
+// Whether rows [tokens, heads, D] of 2-byte elements end before the n at out, or begin after them.
+bool apart(const void* rows, int64_t ts, int64_t hs, int64_t tokens, int64_t heads, int64_t D, const void* out, int64_t n) {
+  const int64_t a = (tokens - 1) * ts, b = (heads - 1) * hs;
+  const int64_t lo = std::min<int64_t>(a, 0) + std::min<int64_t>(b, 0), hi = std::max<int64_t>(a, 0) + std::max<int64_t>(b, 0) + D;
+  const intptr_t r = reinterpret_cast<intptr_t>(rows), o = reinterpret_cast<intptr_t>(out);
+  return r + 2 * hi <= o || r + 2 * lo >= o + 2 * n;
+}
+
 // Launches kern<kT, W> for the row size.
 template <typename Launch>
 void by_width(int D, Launch launch) {
@@ -422,9 +436,11 @@ int check_cache(const MacPagedCache* c, CacheParams& p) {
   return MAC_OK;
 }
 
+// (a launch has fewer than 2^32 threads, a row at most 32 of them)
 int check_items(int64_t tokens, int64_t heads, CacheParams& p) {
+  constexpr int64_t kMost = (int64_t{1} << 27) - 8;
   REQUIRE(tokens >= 0, "tokens must be >= 0");
-  REQUIRE(heads < INT_MAX && tokens <= INT_MAX / heads, "too many rows (tokens * heads must fit 31 bits)");
+  REQUIRE(heads < INT_MAX && tokens <= kMost / heads, "too many rows (tokens * heads must be less than 2^27)");
   p.items = static_cast<uint32_t>(tokens * heads);
   return MAC_OK;
 }
@@ -475,6 +491,12 @@ extern "C" int mac_paged_rope_write_fp8(const MacPagedCache* c, const MacPagedRo
   REQUIRE(a->cos_sin_rows > 0, "cos_sin_cache must not be empty");
   REQUIRE(a->q && a->k && a->v && a->q_out && a->cos_sin_cache && a->positions && a->cache_locs, "null pointer argument");
   REQUIRE(aligned(a->q_out, 16), "q_out must be 16-byte aligned");
+  // (a rotated element's partner is read from the row itself)
+  const int64_t out_n = a->tokens * a->Hq * c->D;
+  REQUIRE(apart(a->q, a->q_stride0, a->q_stride1, a->tokens, a->Hq, c->D, a->q_out, out_n) &&
+              apart(a->k, a->k_stride0, a->k_stride1, a->tokens, c->Hkv, c->D, a->q_out, out_n) &&
+              apart(a->v, a->v_stride0, a->v_stride1, a->tokens, c->Hkv, c->D, a->q_out, out_n),
+          "q_out must not overlap q, k or v");
   p.q = static_cast<const uint16_t*>(a->q);
   p.k = static_cast<const uint16_t*>(a->k);
   p.v = static_cast<const uint16_t*>(a->v);

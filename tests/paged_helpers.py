@@ -47,8 +47,10 @@ def row_bytes(x):
 def quantise(x, scaled, factor=1.0):
     """(codes, bytes or None) of rows x."""
     if not scaled:
-        # (the quotient is an IEEE fp32 division: its rounding is part of the format)
-        return nearest_codes((x.float() / torch.tensor(factor, dtype=torch.float32, device=x.device)).double()), None
+        # (the quotient is an IEEE fp32 division: its rounding is part of the format;
+        # one of a finite x that overflows saturates)
+        y = (x.float() / torch.tensor(factor, dtype=torch.float32, device=x.device)).double()
+        return nearest_codes(torch.where(x.isfinite(), y.clamp(-448.0, 448.0), y)), None
     b = row_bytes(x.double())
     return nearest_codes(x.double() * torch.exp2(127 - b.double())[..., None]), b
 

@@ -152,7 +152,9 @@ def rope_args(bridge, **kw):
     (dict(struct_size=4), "struct_size"), (dict(abi_version=9), "abi_version"), (dict(dtype=F32), "bfloat16 or float16"), (dict(Hq=0), "Hq"),
     (dict(rotary_dim=0), "rotary_dim"), (dict(rotary_dim=7), "rotary_dim"), (dict(rotary_dim=130), "rotary_dim"), (dict(cos_sin_rows=0), "empty"),
     (dict(q=None), "null pointer"), (dict(positions=None), "null pointer"), (dict(q_out=BASE + 8), "16-byte aligned"),
-    (dict(tokens=-1), ">= 0"), (dict(tokens=1 << 31), "too many rows"),
+    (dict(tokens=-1), ">= 0"), (dict(tokens=1 << 31), "too many rows"), (dict(q_out=BASE * 4), "overlap"),
+    (dict(q_out=BASE * 4 + 2032), "overlap"), (dict(q_out=BASE * 5 - 1008), "overlap"), (dict(q_out=BASE * 6 - 2032), "overlap"),
+    (dict(q=BASE * 64, q_stride0=-1024, tokens=3, q_out=BASE * 64 - 4096), "overlap"),
 ])
 def test_rope_writes_refuse(bridge, lib, change, text):
     c = make_cache(bridge)
@@ -197,13 +199,18 @@ def test_attention_refuses_bad_caches(bridge, lib, change, text):
     (dict(logit_cap=1e60), "fit fp32"), (dict(logit_cap=1e-60), "fit fp32"), (dict(q=None), "null pointer"), (dict(out=None), "null pointer"),
     (dict(out_lse=None), "null pointer"), (dict(page_table=None), "null pointer"), (dict(q=BASE + 8), "16-byte aligned"),
     (dict(q_stride0=1020), "16-byte aligned"), (dict(out=BASE + 4), "16-byte aligned"),
-    (dict(total_q=1 << 27, B=4096), "too large"),
+    (dict(total_q=1 << 24, Hq=2), "total_q"), (dict(total_q=(1 << 24) - 1, Hq=64, B=4096), "too large"),
 ])
 def test_attention_refuses(bridge, lib, change, text):
     c = make_cache(bridge)
     refused(lib, attend(lib, c, attention_args(bridge, **change)), text)
     refused(lib, attend(lib, None, attention_args(bridge)), "NULL")
     refused(lib, attend(lib, c, None), "NULL")
+
+
+def test_attention_refuses_more_rows_and_heads_than_a_launch_has_workgroups(bridge, lib):
+    c = make_cache(bridge, Hkv=2048)
+    refused(lib, attend(lib, c, attention_args(bridge, Hq=2048, total_q=512 * 16, B=512)), "batch too large")
 
 
 def test_attention_refuses_small_workspaces(bridge, lib):
