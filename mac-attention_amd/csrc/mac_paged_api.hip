@@ -29,7 +29,7 @@ constexpr int kMaxB = 4096;  // requests handled by the in-workgroup plan
 constexpr int kMaxQ = 1 << 24;  // workgroups: a launch has fewer than 2^32 threads
 
 struct Choice {
-  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = kPlain, by_rows = 0, grid = 0;
+  int body = 0, cols = 0, heads_shift = 0, task_rows = 0, unit_shift = 0, stream = kPlain, spare = 0, by_rows = 0, grid = 0;
   size_t plan_bytes = 0, ml_bytes = 0, o_bytes = 0;
   size_t bytes() const { return plan_bytes + ml_bytes + o_bytes; }
 };
@@ -78,28 +78,28 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   const int64_t worst = static_cast<int64_t>(B) * ((total_q * G + ch.cols - 1) / ch.cols) * c.Hkv;
   if (worst >= INT_MAX) return false;
   const int resident = variant(q_dtype, c.cache_dtype).resident(c.D, ch.body, B);
-  // The tile body streams its keys where its tasks leave part of the GPU idle; else
-  // workgroups that take whole tasks, in step over the same keys, share them in L2 and
-  // write no partial states.  Streamed / whole, 4 heads per group (us): 512 rows over 32K
-  // keys (128 tasks of 512 resident) 354 / 893, over 8K 127 / 240, 1024 over 8K (256) 207 /
-  // 248; 24 ragged requests of 64 dims (592 tasks of 768) 106 / 140; 2048 rows over 2K (512
-  // of 512) 116 / 84, over 8K 364 / 320, 4 x 2048 of 64 dims (1024 of 768) 482 / 408.
-  // The tasks of one request are about as long as each other; of several, the device
-  // looks (paged_plan).
+  // The stream body streams its keys.  The tile body does where whole tasks would leave
+  // much of the GPU idle or take very different times, which the lengths decide, on the
+  // device (paged_plan); else workgroups that take whole tasks, in step over the same
+  // keys, share them in L2 and write no partial states (streamed / whole, 4 heads per
+  // group, us: 2048 rows over 2K keys, 512 tasks of 512 resident, 116 / 84, over 8K 364 /
+  // 320, 4 x 2048 of 64 dims, 1024 of 768, 482 / 408).  One request's tasks are about as
+  // long as each other: enough of them are taken whole.
   const bool fits = 2 * worst < INT_MAX;  // (the units of a task and its partial states)
-  if (ch.body <= kBodyStream32 || tasks < resident) {
+  ch.spare = tasks < resident;
+  if (ch.body <= kBodyStream32) {
     if (!fits) return false;
     ch.stream = kStream;
   } else {
-    ch.stream = B > 1 && fits ? kEither : kPlain;
+    ch.stream = (B > 1 || ch.spare) && fits ? kEither : kPlain;
   }
   ch.grid = resident;
   if (ch.stream == kPlain) {
     ch.grid = static_cast<int>(std::min<int64_t>(tasks, resident));
     return true;
   }
-  // Up to four pieces a task, of many rows: a wave per row and head joins them, else a
-  // workgroup.  Wave / workgroup (us): 24 ragged requests of 64 dims (1.3 pieces) 106 /
+  // Partial states of up to four pieces a task: a wave per row and head joins them, else
+  // a workgroup.  Wave / workgroup (us): 24 ragged requests of 64 dims (1.3 pieces) 106 /
   // 151, 512 rows of 4 heads over 32K keys (4) 373 / 389, 256 (8) 226 / 220, 128 (16) 171
   // / 129, 64 (64) 192 / 86; a token of 256 dims over 8K (256) 144 / 33.
   ch.by_rows = ch.body >= kBodyTile64 && ch.grid <= 4 * tasks;
@@ -215,6 +215,7 @@ extern "C" int mac_paged_chunk_attention(const MacPagedCache* c, const MacPagedA
   p.task_rows = ch.task_rows;
   p.unit_shift = ch.unit_shift;
   p.stream = ch.stream;
+  p.spare = ch.spare;
   p.by_rows = ch.by_rows;
   p.grid = ch.grid;
   const double raw = a->sm_scale * c->k_scale;

@@ -45,6 +45,7 @@ struct PagedParams {
   int task_rows;    // most rows that a task's columns touch
   int unit_shift;   // stream form
   int stream;       // kPlain, kStream or kEither
+  int spare;        // kEither: 1: the tasks leave part of the GPU idle
   int by_rows;      // stream form: 1: partial states combined a row, 0: a row and head per workgroup
   int grid;         // workgroups (stream form: slots hold 2 partials of each)
   float q_scale;    // sm_scale k_scale log2(e); with a cap: 1 (scores are capped to log2 units)
@@ -127,10 +128,15 @@ __device__ __forceinline__ int paged_prefix(PagedArgs& p, bool stream, int* s_pr
 }
 
 // The prefix, and the form: where a choice is left, the stream form if a task is
-// longer than a workgroup's share of the units.  Every workgroup decides alike.  Plain /
-// streamed, 8 KV heads of 4 query heads (us): a chunk of 2048 rows over its own keys and
-// one token over 128K 3365 / 299, and 63 tokens over 16K (a task is as long as the share)
-// 593 / 716; 5 requests of 512 rows over 4K to 32K 990 / 750, 12 such 1717 / 1839.
+// longer than a workgroup's share of the units and 1024 keys more, which pay for the
+// partial states; where whole tasks would leave part of the GPU idle, than one and a
+// half times the share, for a workgroup alone on its CU is the faster one.  Every
+// workgroup decides alike.  Whole / streamed, 8 KV heads of 4 query heads (us): a chunk
+// of 2048 rows over its own keys and one token over 128K 3365 / 299, and 63 tokens over
+// 16K (a task is as long as the share) 593 / 716; 5 requests of 512 rows over 4K to 32K
+// 990 / 750, 12 such 1717 / 1839; part of the GPU: 2 of 334 rows over 500 keys 38 / 62,
+// 2000 79 / 82, 8000 238 / 163; 256 rows over 1000 keys 49 / 61, 2000 77 / 65, 8000 231
+// / 93; 8 of 40 rows over 500 36 / 47, 2000 77 / 61.
 template <bool kEitherForm>
 __device__ __forceinline__ bool paged_plan(PagedArgs& p, int* s_pre, int* s_tmp) {
   if constexpr (!kEitherForm) {
@@ -140,7 +146,8 @@ __device__ __forceinline__ bool paged_plan(PagedArgs& p, int* s_pre, int* s_tmp)
   const int longest = paged_prefix(p, p.stream != kPlain, s_pre, s_tmp);
   if (p.stream != kEither) return p.stream == kStream;
   const int total = s_pre[p.B];
-  if (__syncthreads_or(static_cast<int64_t>(longest) * p.grid > total)) return true;
+  const int more = longest - max(1024 >> p.unit_shift, 1);
+  if (__syncthreads_or(2 * static_cast<int64_t>(more) * p.grid > (2 + p.spare) * static_cast<int64_t>(total))) return true;
   paged_prefix(p, false, s_pre, s_tmp);
   return false;
 }

@@ -1014,6 +1014,7 @@ __global__ void __launch_bounds__(256) combine_kernel(PagedParams, int kc) {
   __shared__ float s_o[4][D], s_m[4], s_l[4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (p.stream == kEither && p.plan[p.B + 1] == 0) return;  // plain form
   const int row = blockIdx.x / p.Hq, head = blockIdx.x - row * p.Hq;
   const int b = request_of_row(p, row);
   if (b < 0) return;
