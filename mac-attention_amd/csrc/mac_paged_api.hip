@@ -84,14 +84,16 @@ bool choose(const MacPagedCache& c, int q_dtype, int Hq, int64_t total_q, int B,
   // keys, share them in L2 and write no partial states (streamed / whole, 4 heads per
   // group, us: 2048 rows over 2K keys, 512 tasks of 512 resident, 116 / 84, over 8K 364 /
   // 320, 4 x 2048 of 64 dims, 1024 of 768, 482 / 408).  One request's tasks are about as
-  // long as each other: enough of them are taken whole.
+  // long as each other: enough of them are taken whole, and so are tasks of tables too
+  // short for the device to stream any (256 rows over their own keys 35 -> 29 without
+  // the combining launch).
   const bool fits = 2 * worst < INT_MAX;  // (the units of a task and its partial states)
   ch.spare = tasks < resident;
   if (ch.body <= kBodyStream32) {
     if (!fits) return false;
     ch.stream = kStream;
   } else {
-    ch.stream = (B > 1 || ch.spare) && fits ? kEither : kPlain;
+    ch.stream = (B > 1 || ch.spare) && fits && max_keys > kShortKeys ? kEither : kPlain;
   }
   ch.grid = resident;
   if (ch.stream == kPlain) {

@@ -13,6 +13,7 @@ namespace mac {
 // Plain form: workgroups take whole tasks in turn.  kEither: the device decides, from
 // the lengths that the host does not know (paged_plan).
 enum { kPlain = 0, kStream = 1, kEither = 2 };
+constexpr int kShortKeys = 1024;  // keys that streaming has to save a workgroup
 
 // What the kernels read.  A call's queries are cut into tasks of `cols`
 // (row, head) columns of one request and KV head; stream form: the tasks' keys
@@ -128,7 +129,7 @@ __device__ __forceinline__ int paged_prefix(PagedArgs& p, bool stream, int* s_pr
 }
 
 // The prefix, and the form: where a choice is left, the stream form if a task is
-// longer than a workgroup's share of the units and 1024 keys more, which pay for the
+// longer than a workgroup's share of the units and kShortKeys more, which pay for the
 // partial states; where whole tasks would leave part of the GPU idle, than one and a
 // half times the share, for a workgroup alone on its CU is the faster one.  Every
 // workgroup decides alike.  Whole / streamed, 8 KV heads of 4 query heads (us): a chunk
@@ -146,7 +147,7 @@ __device__ __forceinline__ bool paged_plan(PagedArgs& p, int* s_pre, int* s_tmp)
   const int longest = paged_prefix(p, p.stream != kPlain, s_pre, s_tmp);
   if (p.stream != kEither) return p.stream == kStream;
   const int total = s_pre[p.B];
-  const int more = longest - max(1024 >> p.unit_shift, 1);
+  const int more = longest - max(kShortKeys >> p.unit_shift, 1);
   if (__syncthreads_or(2 * static_cast<int64_t>(more) * p.grid > (2 + p.spare) * static_cast<int64_t>(total))) return true;
   paged_prefix(p, false, s_pre, s_tmp);
   return false;
